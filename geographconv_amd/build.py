@@ -21,6 +21,8 @@ SOURCES = ['core.hip', 'spmm.hip', 'spmm_hot.hip', 'xt.hip', 'gemm.hip', 'gemm_x
 # (no -munsafe-fp-atomics: the two float atomics of the library -- softmax_adam.hip, exact by construction -- ask for the
 #  hardware add themselves with unsafeAtomicAdd; any future atomicAdd gets the safe default)
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function']
+# no packed fp32 instructions (v_pk_add/mul/fma_f32): some of their forms have given wrong results on this chip, with no error
+FLAGS += ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # ablation / experiment builds: GEOGCN_BUILD_DEFINES="GEOGCN_BF16_PROBE_BUILD ..." python -m geographconv_amd.build --force
 FLAGS += ['-D' + d for d in os.environ.get('GEOGCN_BUILD_DEFINES', '').split()]
 
@@ -32,6 +34,7 @@ def _hipcc():
 def _deps():
     hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
     hdrs.append(os.path.join(os.path.dirname(HERE), 'include', 'geogcn.h'))
+    hdrs.append(os.path.abspath(__file__))                # the flags stand here
     return hdrs
 
 
