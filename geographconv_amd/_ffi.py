@@ -11,8 +11,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libgeogcn.so')
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), 'include', 'geogcn.h')
 
-ACT_NONE, ACT_TANH, ACT_SIGMOID, ACT_SELU, ACT_RELU = 0, 1, 2, 3, 4
+ACT_NONE, ACT_TANH, ACT_SIGMOID, ACT_SELU, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4, 5, 6
 GEMM_F32, GEMM_BF16X3, GEMM_BF16 = 0, 1, 2
+T_F32, T_BF16, T_MX8 = 0, 1, 2
+KEEP_NONE, KEEP_FULL, KEEP_MX8 = 0, 1, 2
 
 c_i32, c_i64, c_f32, c_sz, c_ptr = C.c_int32, C.c_int64, C.c_float, C.c_size_t, C.c_void_p
 c_u64 = C.c_uint64
@@ -124,6 +126,15 @@ SIGNATURES = {
                                      c_i32, c_f32, c_f32, c_ptr]),
     'geogcn_adam_step_ctr_f32': (c_i32, [c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_f32, c_f32, c_f32, c_f32,
                                          c_ptr, c_f32, c_f32, c_ptr]),
+    'geogcn_mx8_pack': (c_i32, [c_i64, c_i32, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr]),
+    'geogcn_mx8_unpack': (c_i32, [c_i64, c_i32, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr]),
+    'geogcn_gated_fwd': (c_i32, [c_i64, c_i64, c_i64, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_i32, c_ptr, c_i64,
+                                 c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i32, c_ptr, C.POINTER(c_sz), c_ptr]),
+    'geogcn_gated_bwd': (c_i32, [c_i64, c_i64, c_i64, c_i32, c_ptr, c_i64, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i32,
+                                 c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr,
+                                 c_i32, c_ptr, C.POINTER(c_sz), c_ptr]),
+    'geogcn_mx8_weight_grad': (c_i32, [c_i64, c_i64, c_i64, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_ptr,
+                                       C.POINTER(c_sz), c_ptr]),
     'geogcn_reg_penalty_f32': (c_i32, [c_i64, c_ptr, c_ptr, c_f32, c_f32, c_ptr, c_ptr, c_sz, c_ptr]),
 }
 

@@ -1,0 +1,970 @@
+// The gated dense block  H = act(X.Wg + bg) * (X.Wu + bu)  and its backward, over fp32, bf16 and 8-bit operands.
+//
+//   forward    [G | U] = X.[Wg | Wu] on the matrix pipe, the activation, the product and (for training) the kept G, U in the epilogue
+//   backward   dG = dH * U * act'(G), dU = dH * act(G)                  one pass, with both bias gradients (gate_grad_kernel)
+//              dX = dG.Wg^T + dU.Wu^T                                   one accumulator over both reductions
+//              [dWg | dWu] = X^T.[dG | dU]                              one launch, X read once
+//
+// All three products run on ONE tiled kernel over bf16 TERMS: an fp32 value is the exact sum of three bf16 values, and a product of two
+// fp32 matrices is the sum of its six largest cross products (the dropped ones are O(2^-24)), accumulated in fp32; a bf16 value is one term
+// and so is an 8-bit checkpoint's (4 significant bits), so X^T.dG from a checkpoint costs three cross products instead of six and loses
+// nothing on the way.  fp32 (and 8-bit) operands are written as term planes [term][row][roundup64(cols)] by terms_kernel or by the pass
+// that forms them; bf16 matrices whose rows are 16-byte aligned are read in place.
+#include "mx8.h"
+
+#include <algorithm>
+
+namespace geogcn {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kOob = 0x80000000u;
+
+// ---- the activation of the gate and its derivative -------------------------------------------------------------------------------------
+__device__ __forceinline__ float gate_value(int act, float x) {
+    switch (act) {
+        case GEOGCN_ACT_SILU: return x * apply_act<GEOGCN_ACT_SIGMOID>(x);
+        case GEOGCN_ACT_GELU: return 0.5f * x * erfcf(-0.70710678118654752f * x);
+        case GEOGCN_ACT_SIGMOID: return apply_act<GEOGCN_ACT_SIGMOID>(x);
+        case GEOGCN_ACT_TANH: return tanhf(x);
+        case GEOGCN_ACT_RELU: return x > 0.f ? x : (x == x ? 0.f : x);
+        default: return x;
+    }
+}
+__device__ __forceinline__ void gate_value_grad(int act, float x, float& v, float& d) {
+    switch (act) {
+        case GEOGCN_ACT_SILU: {
+            const float s = apply_act<GEOGCN_ACT_SIGMOID>(x);
+            v = x * s;
+            d = s * fmaf(x, 1.f - s, 1.f);
+            return;
+        }
+        case GEOGCN_ACT_GELU: {
+            const float cdf = 0.5f * erfcf(-0.70710678118654752f * x);
+            v = x * cdf;
+            d = fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), cdf);
+            return;
+        }
+        case GEOGCN_ACT_SIGMOID: {
+            v = apply_act<GEOGCN_ACT_SIGMOID>(x);
+            d = v * (1.f - v);
+            return;
+        }
+        case GEOGCN_ACT_TANH: {
+            v = tanhf(x);
+            d = fmaf(-v, v, 1.f);
+            return;
+        }
+        case GEOGCN_ACT_RELU: {
+            v = x > 0.f ? x : (x == x ? 0.f : x);
+            d = x > 0.f ? 1.f : 0.f;
+            return;
+        }
+        default: v = x; d = 1.f;
+    }
+}
+
+// ---- a matrix -> its bf16 term planes -----------------------------------------------------------------------------------------------------
+template <int P>
+__global__ __launch_bounds__(256) void terms_kernel(MatIn src, int64_t n, int F, int qpr, uint16_t* __restrict__ out, int64_t ldo, int64_t plane) {
+    const int64_t total = n * qpr;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+        const int64_t r = q / qpr;
+        const int c = (int)(q - r * qpr) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < F) x = mask4(mat_load4_raw(src, r, c), c, F);
+        uint2 t[P];
+        bf16_terms4<P>(x, t);
+#pragma unroll
+        for (int p = 0; p < P; ++p) *reinterpret_cast<uint2*>(out + p * plane + r * ldo + c) = t[p];
+    }
+}
+
+// ---- the tiled product ----------------------------------------------------------------------------------------------------------------------
+// C[m][n] = sum_k A . B over bf16 term planes.  An operand is stored along k (rows = its output dimension, "k-contiguous") or across it (rows =
+// k, "k-strided"): X is k-contiguous in the forward and k-strided in the weight gradient, W the other way round, so nothing is ever
+// transposed in memory.  Stages of BK k-values go straight from global memory to LDS (16 bytes a lane, double-buffered); a k-contiguous image is
+// read as 16-byte fragments, a k-strided one through the transposing LDS read (4 k-values of a lane's own column).  Both images are
+// permuted in 16-byte pieces so that the lanes of a read phase meet different banks.
+// NSEG = 2: the block's columns are BN / 2 of B[0] and the same BN / 2 of B[1] -- a lane then owns g and u of one element.
+struct TileArgs {
+    int64_t M, N;                                     // rows of C, columns of each segment of C
+    int n_mt, n_nt, nsplit, steps_per_split;
+    int n_kseg;
+    int64_t K[2];
+    const uint16_t* A[2]; int64_t lda[2], planeA[2];
+    const uint16_t* B[2]; int64_t ldb[2], planeB[2];
+    // epilogue
+    int mode, out_type, act;
+    void* C[2]; int64_t ldc[2];
+    int64_t ncols;                                    // columns to write (N and the pads kept zero)
+    const float* bias[2];
+    int keep;                                         // EPI_GATED: what is kept of G, U (0, GEOGCN_KEEP_FULL, GEOGCN_KEEP_MX8)
+    void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
+    float* W; int64_t ldw, segw;                      // EPI_SLAB: [split][M][ldw], segment q from column q * segw
+};
+enum { EPI_STORE = 0, EPI_SLAB = 1, EPI_GATED = 2 };
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, int64_t bytes) {
+    const uint32_t n = bytes <= 0 ? 0u : (bytes > 0x7FFFFFFFll ? 0x7FFFFFFFu : (uint32_t)bytes);
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint64_t bu = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
+                        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(bu), 0, __builtin_amdgcn_readfirstlane(n), 0x00020000);
+}
+
+__device__ __forceinline__ void store_quad(void* C, int64_t ld, int type, int64_t row, int64_t col, const float (&x)[4]) {
+    if (type == GEOGCN_T_F32)
+        *reinterpret_cast<float4*>(static_cast<float*>(C) + row * ld + col) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(C) + row * ld + col) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+// One image: R output rows (or columns) by BK k-values of one term plane.
+template <bool STRIDED, int R, int BK>
+struct Image {
+    static constexpr int kBytes = R * BK * 2;
+    static constexpr int kPieces = R * BK / 8;                       // 16-byte pieces
+    static constexpr int kCpr = STRIDED ? R / 8 : BK / 8;            // pieces per stored row
+    static_assert(kPieces % 64 == 0, "whole wave loads");
+    // k-strided: four k-rows of a 16-lane read phase lie a stored row apart -- and a stored row may be a whole round of the banks
+    static __device__ __forceinline__ int rot(int k) {
+        if constexpr ((R * 2) % 256 == 0) return 2 * ((k & 3) + 4 * ((k >> 3) & 1));
+        else if constexpr ((R * 2) % 256 == 128) return 2 * (((k & 3) >> 1) + 2 * ((k >> 3) & 1));
+        else return 2 * ((k >> 3) & 1);
+    }
+    static __device__ __forceinline__ int place(int c, int row) {   // where piece c of stored row `row` lies in that row
+        if constexpr (!STRIDED) return BK == 64 ? (c ^ (row & 7)) : (c ^ ((row >> 1) & 3));
+        else {
+            constexpr bool pow2 = (kCpr & (kCpr - 1)) == 0;
+            if constexpr (pow2) return (c + rot(row)) & (kCpr - 1);
+            int p = c + rot(row);
+            return p >= kCpr ? p - kCpr : p;
+        }
+    }
+    static __device__ __forceinline__ int unplace(int p, int row) {
+        if constexpr (!STRIDED) return place(p, row);
+        else {
+            constexpr bool pow2 = (kCpr & (kCpr - 1)) == 0;
+            if constexpr (pow2) return (p - rot(row)) & (kCpr - 1);
+            const int c = p - rot(row);
+            return c < 0 ? c + kCpr : c;
+        }
+    }
+    // byte offset, from the image's first row and k, of the piece that belongs at place `piece` of the image (kOob: nothing there)
+    static __device__ __forceinline__ uint32_t source(int piece, int64_t ld, int64_t k_left) {
+        const int row = piece / kCpr, c = unplace(piece - row * kCpr, row);
+        if constexpr (STRIDED) return (uint32_t)row * (uint32_t)(ld * 2) + (uint32_t)c * 16u;      // (rows behind the last k: past the descriptor's end)
+        else return c * 8 < k_left ? (uint32_t)row * (uint32_t)(ld * 2) + (uint32_t)c * 16u : kOob;
+    }
+    // the fragment of 16 rows from r0: lane (li, lg) gets its row's k-values s*32 + lg*8 .. + 7
+    static __device__ __forceinline__ bf16x8 read(const unsigned char* img, int r0, int s, int li, int lg) {
+        if constexpr (!STRIDED) {
+            const int row = r0 + li;
+            return *reinterpret_cast<const bf16x8*>(img + row * (BK * 2) + place(s * 4 + lg, row) * 16);
+        } else {
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            const int k = s * 32 + lg * 8 + (li >> 2), c = r0 / 8 + ((li & 3) >> 1);
+            const uint32_t a = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)img + (uint32_t)(k * (R * 2) + place(c, k) * 16 + (li & 1) * 8);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)a);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(a + 4 * R * 2));       // (rot(k + 4) == rot(k))
+            return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+    }
+};
+
+template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, bool GATED>
+__global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
+    constexpr int NW = WM * WN;
+    constexpr int BNS = BN / NSEG;                            // columns of a segment
+    typedef Image<ASTR, BM, BK> IA;
+    typedef Image<BSTR, BNS, BK> IB;
+    constexpr int MT = BM / WM / 16;                          // 16-row tiles of a wave
+    constexpr int CW = BNS / WN, NTS = CW / 16, NT = NTS * NSEG;
+    static_assert(BM % (WM * 16) == 0 && CW % 16 == 0 && (!GATED || (NSEG == 2 && CW % 32 == 0)), "wave tiles");
+    constexpr int kA = PA * IA::kBytes, kStage = kA + PB * NSEG * IB::kBytes;
+    constexpr int LA = PA * IA::kPieces / 64, LB = PB * NSEG * IB::kPieces / 64, LOADS = LA + LB;      // wave loads of a stage
+    extern __shared__ __attribute__((aligned(128))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4, wm = wid / WN, wn = wid % WN;
+
+    // tile of this block: every XCD works on a run of neighbouring tiles (blocks go round the XCDs one by one), taken in groups of 8 row tiles
+    // so that the operands of the tiles in flight fit that XCD's L2
+    const int tiles = a.n_mt * a.n_nt, total = tiles * a.nsplit;
+    int id;
+    {
+        const int x = blockIdx.x % kNumXCD, q = total / kNumXCD, r = total % kNumXCD;
+        id = x * q + min(x, r) + (int)blockIdx.x / kNumXCD;
+    }
+    const int z = id / tiles;
+    id -= z * tiles;
+    const int grp = id / (8 * a.n_nt), first = grp * 8, rows_in = min(8, a.n_mt - first), in = id - grp * 8 * a.n_nt;
+    const int mt = first + in % rows_in, nt = in / rows_in;
+    const int64_t m0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNS;
+
+    const int ns0 = (int)((a.K[0] + BK - 1) / BK), nsteps = ns0 + (a.n_kseg == 2 ? (int)((a.K[1] + BK - 1) / BK) : 0);
+    const int t0 = z * a.steps_per_split, t1 = min(nsteps, t0 + a.steps_per_split);
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto issue = [&](int t, int buf) __attribute__((always_inline)) {
+        const int ks = t >= ns0 ? 1 : 0;
+        const int64_t k0 = (int64_t)(ks ? t - ns0 : t) * BK, Kl = (ks ? a.K[1] : a.K[0]) - k0;
+        const int64_t lda = ks ? a.lda[1] : a.lda[0], ldb0 = ks ? a.ldb[1] : a.ldb[0];
+#pragma unroll
+        for (int i = 0; i < (LOADS + NW - 1) / NW; ++i) {
+            const int l = i * NW + wid;
+            if (LOADS % NW != 0 && l >= LOADS) break;
+            const bool isA = LB == 0 || l < LA;
+            const uint16_t* base;
+            int64_t left;                                     // elements from `base` to the end of the plane
+            uint32_t voff;
+            if (isA) {
+                const int p = l / (IA::kPieces / 64), sub = l - p * (IA::kPieces / 64);
+                base = (ks ? a.A[1] : a.A[0]) + p * (ks ? a.planeA[1] : a.planeA[0]);
+                if constexpr (ASTR) { base += k0 * lda + m0; left = Kl * lda - m0; }
+                else { base += m0 * lda + k0; left = (a.M - m0) * lda - k0; }
+                voff = IA::source(sub * 64 + lane, lda, Kl);
+            } else {
+                const int lb = l - LA;
+                const int img = lb / (IB::kPieces / 64), sub = lb - img * (IB::kPieces / 64), sg = NSEG == 2 ? img / PB : 0, p = img - sg * PB;
+                const int w = NSEG == 2 ? sg : ks;
+                const int64_t ldb = NSEG == 2 ? (sg ? a.ldb[1] : a.ldb[0]) : ldb0;
+                base = (w ? a.B[1] : a.B[0]) + p * (w ? a.planeB[1] : a.planeB[0]);
+                if constexpr (BSTR) { base += k0 * ldb + n0; left = Kl * ldb - n0; }
+                else { base += n0 * ldb + k0; left = (a.N - n0) * ldb - k0; }
+                voff = IB::source(sub * 64 + lane, ldb, Kl);
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(base, left * 2), (__attribute__((address_space(3))) void*)(lds + buf * kStage + l * 1024),
+                                                     16, (int)voff, 0, 0, 0);
+        }
+    };
+
+    if (t0 < t1) issue(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        __syncthreads();                                      // stage t has landed, and nobody reads the other buffer any more
+        if (t + 1 < t1) issue(t + 1, buf ^ 1);
+        const unsigned char* As = lds + buf * kStage;
+        const unsigned char* Bs = As + kA;
+#pragma unroll
+        for (int s = 0; s < BK / 32; ++s) {
+            bf16x8 af[MT][PA], bf[NT][PB];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int p = 0; p < PA; ++p) af[i][p] = IA::read(As + p * IA::kBytes, (wm * MT + i) * 16, s, li, lg);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int p = 0; p < PB; ++p)
+                    bf[j][p] = IB::read(Bs + ((j / NTS) * PB + p) * IB::kBytes, wn * CW + (j % NTS) * 16, s, li, lg);
+            // cross products, smallest first; operands swapped, so that a lane owns 4 consecutive columns of one row of C
+#define GEOGCN_TERM(pa, pb)                                                       \
+    _Pragma("unroll") for (int i = 0; i < MT; ++i) _Pragma("unroll") for (int j = 0; j < NT; ++j) \
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][pb], af[i][pa], acc[i][j], 0, 0, 0);
+            if constexpr (PA == 3 && PB == 3) {
+                GEOGCN_TERM(2, 0) GEOGCN_TERM(0, 2) GEOGCN_TERM(1, 1) GEOGCN_TERM(1, 0) GEOGCN_TERM(0, 1)
+            } else if constexpr (PB == 3) {
+                GEOGCN_TERM(0, 2) GEOGCN_TERM(0, 1)
+            }
+            GEOGCN_TERM(0, 0)
+#undef GEOGCN_TERM
+        }
+    }
+
+    // ---- epilogue ----
+    if constexpr (GATED) {
+        if (a.mode == EPI_GATED) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int64_t row = m0 + (wm * MT + i) * 16 + li;
+#pragma unroll
+                for (int jj = 0; jj < NTS; jj += 2) {
+                    float v[2][2][4];                         // [g, u][16-column tile][column]: 32 columns = one block of a checkpoint
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int64_t col = n0 + wn * CW + (jj + h) * 16 + lg * 4;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float* b = a.bias[q];
+                                v[q][h][r] = col + r < a.N ? acc[i][q * NTS + jj + h][r] + (b ? b[col + r] : 0.f) : 0.f;
+                            }
+                    }
+                    if (row < a.M) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int64_t col = n0 + wn * CW + (jj + h) * 16 + lg * 4;
+                            if (col < a.ncols) {
+                                float x[4];
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) x[r] = col + r < a.N ? gate_value(a.act, v[0][h][r]) * v[1][h][r] : 0.f;
+                                store_quad(a.C[0], a.ldc[0], a.out_type, row, col, x);
+                                if (a.keep == GEOGCN_KEEP_FULL) {
+                                    store_quad(a.keepP[0], a.ldk[0], a.out_type, row, col, v[0][h]);
+                                    store_quad(a.keepP[1], a.ldk[1], a.out_type, row, col, v[1][h]);
+                                }
+                            }
+                        }
+                    }
+                    if (a.keep == GEOGCN_KEEP_MX8) {
+                        const int64_t c0 = n0 + wn * CW + jj * 16;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t m = 0;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) m = max(m, mx8_abs_bits(v[q][h][r]));
+                            m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+                            m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+                            const uint32_t b = mx8_scale_byte(m);
+                            const float inv = mx8_inv_scale(b);
+                            if (row < a.M && c0 < a.N) {
+                                uint8_t* codes = static_cast<uint8_t*>(a.keepP[q]) + row * a.ldk[q] + c0;
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    *reinterpret_cast<uint32_t*>(codes + h * 16 + lg * 4) =
+                                        mx8_encode4(v[q][h][0], v[q][h][1], v[q][h][2], v[q][h][3], inv, b != 255u);
+                                if (lg == 0) a.keepS[q][row * (a.ldk[q] / kMxBlock) + c0 / kMxBlock] = (uint8_t)b;
+                            }
+                        }
+                    }
+                }
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t row = m0 + (wm * MT + i) * 16 + li;
+        if (row >= a.M) continue;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int q = j / NTS;
+            const int64_t col = n0 + wn * CW + (j % NTS) * 16 + lg * 4;
+            float x[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = col + r < a.N ? acc[i][j][r] : 0.f;
+            if (a.mode == EPI_SLAB) {
+                if (col < a.segw) *reinterpret_cast<float4*>(a.W + ((int64_t)z * a.M + row) * a.ldw + q * a.segw + col) = make_float4(x[0], x[1], x[2], x[3]);
+            } else if (col < a.ncols) {
+                store_quad(a.C[q], a.ldc[q], a.out_type, row, col, x);
+            }
+        }
+    }
+}
+
+// ---- partial products of a split reduction, added in split order, and the epilogue that they were waiting for ---------------------------
+struct FinishArgs {
+    int64_t M, N, segw, ldw, ncols;
+    int nsplit, nseg, mode, out_type, act, keep;
+    const float* W;
+    void* C[2]; int64_t ldc[2];
+    const float* bias[2];
+    void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
+};
+__global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
+    // quads of columns; in the gated epilogue whole checkpoint blocks of 8 lanes stay together (segw is a multiple of 32)
+    const int64_t qpr = a.segw / 4, total = a.M * qpr;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        const int64_t row = e / qpr, col = (e - row * qpr) * 4;
+        float v[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if (q >= a.nseg) break;
+            const float* w = a.W + row * a.ldw + q * a.segw + col;
+            for (int z = 0; z < a.nsplit; ++z) {
+                const float4 t = *reinterpret_cast<const float4*>(w + (int64_t)z * a.M * a.ldw);
+                v[q][0] += t.x; v[q][1] += t.y; v[q][2] += t.z; v[q][3] += t.w;
+            }
+        }
+        if (a.mode != EPI_GATED) {
+            if (col < a.ncols)
+                for (int q = 0; q < a.nseg; ++q) store_quad(a.C[q], a.ldc[q], a.out_type, row, col, v[q]);
+            continue;
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[q][r] = col + r < a.N ? v[q][r] + (a.bias[q] ? a.bias[q][col + r] : 0.f) : 0.f;
+        if (col < a.ncols) {
+            float x[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = col + r < a.N ? gate_value(a.act, v[0][r]) * v[1][r] : 0.f;
+            store_quad(a.C[0], a.ldc[0], a.out_type, row, col, x);
+            if (a.keep == GEOGCN_KEEP_FULL)
+                for (int q = 0; q < 2; ++q) store_quad(a.keepP[q], a.ldk[q], a.out_type, row, col, v[q]);
+        }
+        if (a.keep == GEOGCN_KEEP_MX8) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t m = max(max(mx8_abs_bits(v[q][0]), mx8_abs_bits(v[q][1])), max(mx8_abs_bits(v[q][2]), mx8_abs_bits(v[q][3])));
+                m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+                m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+                m = max(m, (uint32_t)__shfl_xor((int)m, 4));
+                const uint32_t b = mx8_scale_byte(m);
+                if (col / kMxBlock * kMxBlock < a.N) {
+                    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.keepP[q]) + row * a.ldk[q] + col) =
+                        mx8_encode4(v[q][0], v[q][1], v[q][2], v[q][3], mx8_inv_scale(b), b != 255u);
+                    if (col % kMxBlock == 0) a.keepS[q][row * (a.ldk[q] / kMxBlock) + col / kMxBlock] = (uint8_t)b;
+                }
+            }
+        }
+    }
+}
+
+// ---- dG, dU as term planes (P = 0: as fp32 matrices), with the partial column sums of both (bias gradients) ------------------------------
+constexpr int kGradRows = 128;          // rows of a block: its partial sums are 32 sequential adds per wave, then a tree
+template <int P>
+__global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn U, int64_t M, int N, int act, uint16_t* __restrict__ oG,
+                                                        uint16_t* __restrict__ oU, int64_t ldo, int64_t plane, float* __restrict__ part, int64_t part_ld) {
+    __shared__ float red[4][64][8];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int c = (blockIdx.x * 64 + lane) * 4;
+    const int64_t r0 = (int64_t)blockIdx.y * kGradRows, r1 = min(M, r0 + kGradRows);
+    float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < ldo) {
+        for (int64_t r = r0 + w; r < r1; r += 4) {
+            float4 dg = make_float4(0.f, 0.f, 0.f, 0.f), du = dg;
+            if (c < N) {
+                const float4 d = mat_load4_raw(dH, r, c), g = mat_load4_raw(G, r, c), u = mat_load4_raw(U, r, c);
+                const float dv[4] = {d.x, d.y, d.z, d.w}, gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
+                float og[4], ou[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v, s;
+                    gate_value_grad(act, gv[k], v, s);
+                    og[k] = dv[k] * uv[k] * s;
+                    ou[k] = dv[k] * v;
+                }
+                dg = mask4(make_float4(og[0], og[1], og[2], og[3]), c, N);
+                du = mask4(make_float4(ou[0], ou[1], ou[2], ou[3]), c, N);
+            }
+            sg[0] += dg.x; sg[1] += dg.y; sg[2] += dg.z; sg[3] += dg.w;
+            su[0] += du.x; su[1] += du.y; su[2] += du.z; su[3] += du.w;
+            if constexpr (P == 0) {
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(oG) + r * ldo + c) = dg;
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(oU) + r * ldo + c) = du;
+            } else {
+                uint2 tg[P], tu[P];
+                bf16_terms4<P>(dg, tg);
+                bf16_terms4<P>(du, tu);
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    *reinterpret_cast<uint2*>(oG + p * plane + r * ldo + c) = tg[p];
+                    *reinterpret_cast<uint2*>(oU + p * plane + r * ldo + c) = tu[p];
+                }
+            }
+        }
+    }
+    if (!part) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { red[w][lane][k] = sg[k]; red[w][lane][4 + k] = su[k]; }
+    __syncthreads();
+    if (w < 2 && c < N) {
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] = (red[0][lane][w * 4 + k] + red[1][lane][w * 4 + k]) + (red[2][lane][w * 4 + k] + red[3][lane][w * 4 + k]);
+        *reinterpret_cast<float4*>(part + ((int64_t)w * gridDim.y + blockIdx.y) * part_ld + c) = make_float4(s[0], s[1], s[2], s[3]);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------------------
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// bump allocator over the caller's workspace; with base == nullptr it only counts
+struct Arena {
+    unsigned char* base;
+    size_t used = 0;
+    void* take(int64_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += (size_t)up(bytes, 256);
+        return p;
+    }
+};
+
+// an operand as the tiled kernel reads it
+struct Planes { const uint16_t* p; int64_t ld, plane; };
+
+// in place where a bf16 matrix's rows start on 16 bytes (and its k-extent is whole pieces, `whole_cols`), else term planes in the workspace
+int make_planes(Arena& ar, const MatIn& m, int64_t n, int64_t F, int P, bool whole_cols, hipStream_t st, Planes* out) {
+    if (m.type == GEOGCN_T_BF16 && m.ld % 8 == 0 && aligned16(m.p) && (!whole_cols || F % 8 == 0)) {
+        *out = Planes{static_cast<const uint16_t*>(m.p), m.ld, 0};
+        return 0;
+    }
+    const int64_t ld = up(F, 64), plane = n * ld;
+    uint16_t* o = static_cast<uint16_t*>(ar.take(plane * 2 * P));
+    *out = Planes{o, ld, plane};
+    if (!ar.base || plane == 0) return 0;
+    const int qpr = (int)(ld / 4);
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(n * qpr, 256), (int64_t)kNumCU * 32);
+    if (P == 3) hipLaunchKernelGGL(terms_kernel<3>, dim3(grid), dim3(256), 0, st, m, n, (int)F, qpr, o, ld, plane);
+    else hipLaunchKernelGGL(terms_kernel<1>, dim3(grid), dim3(256), 0, st, m, n, (int)F, qpr, o, ld, plane);
+    GEOGCN_LAUNCH_CHECK("terms_kernel");
+    return 0;
+}
+
+template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, bool GATED>
+int launch_tile(const TileArgs& a, hipStream_t st) {
+    constexpr int bytes = 2 * BK * 2 * (PA * BM + PB * BN);
+    static LdsAttrOnce attr;
+    auto* k = &tile_kernel<PA, PB, ASTR, BSTR, NSEG, BM, BN, BK, WM, WN, GATED>;
+    if (const int rc = attr.ensure(reinterpret_cast<const void*>(k), bytes)) return rc;
+    hipLaunchKernelGGL(k, dim3((unsigned)(a.n_mt * a.n_nt * a.nsplit)), dim3(WM * WN * 64), bytes, st, a);
+    GEOGCN_LAUNCH_CHECK("tile_kernel");
+    return 0;
+}
+
+// how a product is cut: tiles of the output, and its reduction over `nsplit` blocks where the tiles alone leave CUs idle
+struct Cut { int n_mt, n_nt, nsplit, steps; };
+Cut cut_of(int64_t M, int64_t ncols, int64_t bm, int64_t bns, int64_t steps) {
+    Cut c;
+    c.n_mt = (int)cdiv(M, bm);
+    c.n_nt = (int)cdiv(ncols, bns);
+    const int64_t tiles = (int64_t)c.n_mt * c.n_nt;
+    int64_t want = tiles >= kNumCU ? 1 : kNumCU / tiles;
+    want = std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));             // at least four stages a block
+    c.steps = (int)cdiv(std::max<int64_t>(steps, 1), want);
+    c.nsplit = (int)std::max<int64_t>(1, cdiv(steps, c.steps));
+    return c;
+}
+
+int64_t out_cols(int type, int64_t N, int64_t ld) { return std::min<int64_t>(ld, up(N, type == GEOGCN_T_F32 ? 4 : 64)); }
+
+int finish(const TileArgs& t, int nseg, int mode, hipStream_t st) {
+    FinishArgs f;
+    f.M = t.M; f.N = t.N; f.segw = t.segw; f.ldw = t.ldw; f.ncols = t.ncols;
+    f.nsplit = t.nsplit; f.nseg = nseg; f.mode = mode; f.out_type = t.out_type; f.act = t.act; f.keep = t.keep;
+    f.W = t.W;
+    for (int q = 0; q < 2; ++q) {
+        f.C[q] = t.C[q]; f.ldc[q] = t.ldc[q]; f.bias[q] = t.bias[q];
+        f.keepP[q] = t.keepP[q]; f.ldk[q] = t.ldk[q]; f.keepS[q] = t.keepS[q];
+    }
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(t.M * (t.segw / 4), 256), (int64_t)kNumCU * 32);
+    hipLaunchKernelGGL(finish_kernel, dim3(grid), dim3(256), 0, st, f);
+    GEOGCN_LAUNCH_CHECK("finish_kernel");
+    return 0;
+}
+
+// X.[Wg | Wu] and the gate
+int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
+    constexpr int BM = 128, BNS = 128;
+    const int64_t bk = P == 3 ? 32 : 64;
+    const Cut c = cut_of(t.M, std::max(t.ncols, t.keep == GEOGCN_KEEP_MX8 ? up(t.N, kMxBlock) : 0), BM, BNS, cdiv(t.K[0], bk));
+    t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
+    t.segw = (int64_t)c.n_nt * BNS; t.ldw = 2 * t.segw;
+    if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
+    if (!ar.base) return 0;
+    t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_GATED;
+    const int rc = P == 3 ? launch_tile<3, 3, false, true, 2, BM, 2 * BNS, 32, 2, 4, true>(t, st)
+                          : launch_tile<1, 1, false, true, 2, BM, 2 * BNS, 64, 2, 4, true>(t, st);
+    if (rc || c.nsplit == 1) return rc;
+    return finish(t, 2, EPI_GATED, st);
+}
+
+// dG.Wg^T + dU.Wu^T
+int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
+    constexpr int BM = 128, BN = 128;
+    const int64_t bk = P == 3 ? 32 : 64;
+    const Cut c = cut_of(t.M, t.ncols, BM, BN, 2 * cdiv(t.K[0], bk));
+    t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
+    t.segw = (int64_t)c.n_nt * BN; t.ldw = t.segw;
+    if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
+    if (!ar.base) return 0;
+    t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_STORE;
+    const int rc = P == 3 ? launch_tile<3, 3, false, false, 1, BM, BN, 32, 2, 2, false>(t, st)
+                          : launch_tile<1, 1, false, false, 1, BM, BN, 64, 2, 2, false>(t, st);
+    if (rc || c.nsplit == 1) return rc;
+    return finish(t, 1, EPI_STORE, st);
+}
+
+// X^T.[B0 | B1] (nseg = 2) or X^T.B0
+int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_t st) {
+    constexpr int BM = 128, BNS = 128;
+    const int64_t bk = PB == 3 ? 32 : 64;
+    const Cut c = cut_of(t.M, t.ncols, BM, BNS, cdiv(t.K[0], bk));
+    t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
+    t.segw = (int64_t)c.n_nt * BNS; t.ldw = nseg * t.segw;
+    if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
+    if (!ar.base) return 0;
+    t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_STORE;
+    int rc;
+    if (nseg == 2) {
+        if (PA == 3) rc = launch_tile<3, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, false>(t, st);
+        else if (PB == 3) rc = launch_tile<1, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, false>(t, st);
+        else rc = launch_tile<1, 1, true, true, 2, BM, 2 * BNS, 64, 2, 4, false>(t, st);
+    } else {
+        if (PB == 3) rc = launch_tile<1, 3, true, true, 1, BM, BNS, 32, 2, 4, false>(t, st);
+        else rc = launch_tile<1, 1, true, true, 1, BM, BNS, 64, 2, 4, false>(t, st);
+    }
+    if (rc || c.nsplit == 1) return rc;
+    return finish(t, nseg, EPI_STORE, st);
+}
+
+TileArgs tile_args() {
+    TileArgs t;
+    memset(&t, 0, sizeof(t));
+    t.n_kseg = 1;
+    return t;
+}
+
+int elem_align(int type) { return type == GEOGCN_T_F32 ? 16 : type == GEOGCN_T_BF16 ? 8 : 4; }
+
+int check_mat(const char* who, const char* name, int type, const void* p, int64_t ld, const uint8_t* scale, int64_t F) {
+    GEOGCN_REQUIRE(p, GEOGCN_E_NULL, "%s: %s is null", who, name);
+    GEOGCN_REQUIRE(reinterpret_cast<uintptr_t>(p) % elem_align(type) == 0, GEOGCN_E_ALIGN, "%s: %s is not aligned", who, name);
+    if (type == GEOGCN_T_MX8) {
+        GEOGCN_REQUIRE(scale, GEOGCN_E_NULL, "%s: %s has no scales", who, name);
+        GEOGCN_REQUIRE(ld % kMxBlock == 0 && ld >= F, GEOGCN_E_ALIGN, "%s: code pitch %lld of %s (%lld columns) is not whole blocks", who,
+                       (long long)ld, name, (long long)F);
+    } else {
+        GEOGCN_REQUIRE(ld % 4 == 0 && ld >= up(F, 4), GEOGCN_E_ALIGN, "%s: pitch %lld of %s (%lld columns)", who, (long long)ld, name, (long long)F);
+    }
+    return 0;
+}
+
+bool act_ok(int act) {
+    return act == GEOGCN_ACT_NONE || act == GEOGCN_ACT_TANH || act == GEOGCN_ACT_SIGMOID || act == GEOGCN_ACT_RELU || act == GEOGCN_ACT_SILU ||
+           act == GEOGCN_ACT_GELU;
+}
+
+// terms per value of an operand: bf16 and 8-bit values are one term; fp32 three, or one (rounded) where the caller asked for bf16 products
+int terms_of(int type, int precision) { return type == GEOGCN_T_F32 && precision != GEOGCN_GEMM_BF16 ? 3 : 1; }
+
+int check_dims(const char* who, int64_t M, int64_t K, int64_t N) {
+    GEOGCN_REQUIRE(M >= 0 && K >= 0 && N >= 0, GEOGCN_E_SIZE, "%s: negative size", who);
+    GEOGCN_REQUIRE(K <= (1 << 20) && N <= (1 << 20) && M <= (int64_t)1 << 31, GEOGCN_E_SIZE, "%s: %lld x %lld -> %lld is too large", who, (long long)M,
+                   (long long)K, (long long)N);
+    return 0;
+}
+
+struct FwdArgs {
+    int64_t M, K, N;
+    int type, precision, keep, act;
+    MatIn X, Wg, Wu;
+    const float *bg, *bu;
+    void* H; int64_t ldh;
+    void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
+};
+int forward_exact(Arena& ar, const FwdArgs& f, hipStream_t st) {
+    // [G | U] by the library's dual product into one slab, the gate by the pass that finishes split reductions
+    TileArgs t = tile_args();
+    t.M = f.M; t.N = f.N; t.nsplit = 1;
+    t.segw = up(f.N, kMxBlock); t.ldw = 2 * t.segw;
+    t.W = static_cast<float*>(ar.take(f.M * t.ldw * 4));
+    t.out_type = f.type; t.act = f.act; t.keep = f.keep;
+    t.C[0] = f.H; t.ldc[0] = f.ldh; t.ncols = out_cols(f.type, f.N, f.ldh);
+    t.bias[0] = f.bg; t.bias[1] = f.bu;
+    for (int q = 0; q < 2; ++q) { t.keepP[q] = f.keepP[q]; t.ldk[q] = f.ldk[q]; t.keepS[q] = f.keepS[q]; }
+    const size_t need = f.K ? geogcn_gemm_dual_workspace_bytes(0, f.M, f.N, f.N, f.K, GEOGCN_GEMM_F32) : 0;
+    void* w = ar.take((int64_t)need);
+    if (!ar.base) return 0;
+    if (f.K == 0) {
+        if (const int rc = zero_rows_async(t.W, f.M, t.ldw, t.ldw, st)) return rc;
+    } else if (const int rc = geogcn_gemm_dual_f32(0, f.M, f.N, f.N, f.K, static_cast<const float*>(f.X.p), f.X.ld, static_cast<const float*>(f.Wg.p),
+                                                   f.Wg.ld, static_cast<const float*>(f.Wu.p), f.Wu.ld, t.W, t.ldw, t.W + t.segw, t.ldw, nullptr,
+                                                   GEOGCN_ACT_NONE, nullptr, GEOGCN_ACT_NONE, GEOGCN_GEMM_F32, need ? w : nullptr, need, st)) return rc;
+    return finish(t, 2, EPI_GATED, st);
+}
+int forward(Arena& ar, const FwdArgs& f, hipStream_t st) {
+    if (f.precision == GEOGCN_GEMM_F32 && f.type == GEOGCN_T_F32) return forward_exact(ar, f, st);
+    const int P = terms_of(f.type, f.precision);
+    Planes x, wg, wu;
+    if (const int rc = make_planes(ar, f.X, f.M, f.K, P, true, st, &x)) return rc;
+    if (const int rc = make_planes(ar, f.Wg, f.K, f.N, P, false, st, &wg)) return rc;
+    if (const int rc = make_planes(ar, f.Wu, f.K, f.N, P, false, st, &wu)) return rc;
+    TileArgs t = tile_args();
+    t.M = f.M; t.N = f.N; t.K[0] = f.K;
+    t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
+    t.B[0] = wg.p; t.ldb[0] = wg.ld; t.planeB[0] = wg.plane;
+    t.B[1] = wu.p; t.ldb[1] = wu.ld; t.planeB[1] = wu.plane;
+    t.out_type = f.type; t.act = f.act; t.keep = f.keep;
+    t.C[0] = f.H; t.ldc[0] = f.ldh;
+    t.ncols = out_cols(f.type, f.N, f.ldh);
+    t.bias[0] = f.bg; t.bias[1] = f.bu;
+    for (int q = 0; q < 2; ++q) { t.keepP[q] = f.keepP[q]; t.ldk[q] = f.ldk[q]; t.keepS[q] = f.keepS[q]; }
+    return run_forward(ar, t, P, st);
+}
+
+struct BwdArgs {
+    int64_t M, K, N;
+    int type, precision, act;
+    MatIn dH, X, G, U, Wg, Wu;
+    void *dX; int64_t lddx;
+    void* dW[2]; int64_t lddw[2];
+    float* db[2];
+};
+// P = 0: dG, dU as fp32 matrices of pitch ldo
+int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t st, uint16_t** dG_out, uint16_t** dU_out) {
+    const int64_t plane = b.M * ldo, bytes = P ? plane * 2 * P : plane * 4;
+    uint16_t* dG = *dG_out = static_cast<uint16_t*>(ar.take(bytes));
+    uint16_t* dU = *dU_out = static_cast<uint16_t*>(ar.take(bytes));
+    const int64_t nparts = cdiv(b.M, kGradRows), part_ld = up(b.N, 4);
+    float* part = b.db[0] ? static_cast<float*>(ar.take(2 * nparts * part_ld * 4)) : nullptr;
+    if (ar.base) {
+        const dim3 grid((unsigned)cdiv(ldo, 256), (unsigned)nparts);
+        auto* k = P == 3 ? &gate_grad_kernel<3> : P == 1 ? &gate_grad_kernel<1> : &gate_grad_kernel<0>;
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, ldo, plane, part, part_ld);
+        GEOGCN_LAUNCH_CHECK("gate_grad_kernel");
+        if (part)
+            for (int q = 0; q < 2; ++q)
+                if (const int rc = colsum_final_launch((int)nparts, (int)b.N, part + q * nparts * part_ld, part_ld, b.db[q], st)) return rc;
+    }
+    return 0;
+}
+// the products by the library's fp32 kernels: dG, dU (and a checkpointed X) as fp32 matrices
+int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
+    const int64_t ldo = up(b.N, 4);
+    uint16_t *g, *u;
+    if (const int rc = gate_gradients(ar, b, 0, ldo, st, &g, &u)) return rc;
+    const float *dG = reinterpret_cast<const float*>(g), *dU = reinterpret_cast<const float*>(u);
+    if (b.dX) {
+        const size_t need = geogcn_gemm_kcat_workspace_bytes(1, b.M, b.K, b.N, b.N, precision);
+        void* w = ar.take((int64_t)need);
+        if (ar.base)
+            if (const int rc = geogcn_gemm_kcat_f32(1, b.M, b.K, b.N, b.N, dG, ldo, static_cast<const float*>(b.Wg.p), b.Wg.ld, dU, ldo,
+                                                    static_cast<const float*>(b.Wu.p), b.Wu.ld, static_cast<float*>(b.dX), b.lddx, 0, precision,
+                                                    need ? w : nullptr, need, st)) return rc;
+    }
+    if (b.dW[0]) {
+        const float* X = static_cast<const float*>(b.X.p);
+        int64_t ldx = b.X.ld;
+        if (b.X.type == GEOGCN_T_MX8) {
+            ldx = up(b.K, 4);
+            float* x = static_cast<float*>(ar.take(b.M * ldx * 4));
+            if (ar.base)
+                if (const int rc = geogcn_mx8_unpack(b.M, (int32_t)b.K, GEOGCN_T_F32, static_cast<const uint8_t*>(b.X.p), b.X.ld, b.X.scale, x, ldx, st)) return rc;
+            X = x;
+        }
+        const size_t need = geogcn_gemm_dual_workspace_bytes(1, b.K, b.N, b.N, b.M, precision);
+        void* w = ar.take((int64_t)need);
+        if (ar.base)
+            if (const int rc = geogcn_gemm_dual_f32(1, b.K, b.N, b.N, b.M, X, ldx, dG, ldo, dU, ldo, static_cast<float*>(b.dW[0]), b.lddw[0],
+                                                    static_cast<float*>(b.dW[1]), b.lddw[1], nullptr, GEOGCN_ACT_NONE, nullptr, GEOGCN_ACT_NONE, precision,
+                                                    need ? w : nullptr, need, st)) return rc;
+    }
+    return 0;
+}
+int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
+    if (b.precision == GEOGCN_GEMM_F32 && b.type == GEOGCN_T_F32) return backward_exact(ar, b, GEOGCN_GEMM_F32, st);
+    const int P = terms_of(b.type, b.precision), PX = b.X.type == GEOGCN_T_F32 ? P : 1;
+    const int64_t ldo = up(b.N, 64), plane = b.M * ldo;
+    uint16_t *dG, *dU;
+    if (const int rc = gate_gradients(ar, b, P, ldo, st, &dG, &dU)) return rc;
+    if (b.dX) {
+        Planes wg, wu;
+        if (const int rc = make_planes(ar, b.Wg, b.K, b.N, P, true, st, &wg)) return rc;
+        if (const int rc = make_planes(ar, b.Wu, b.K, b.N, P, true, st, &wu)) return rc;
+        TileArgs t = tile_args();
+        t.M = b.M; t.N = b.K; t.n_kseg = 2; t.K[0] = t.K[1] = b.N;
+        t.A[0] = dG; t.A[1] = dU;
+        t.B[0] = wg.p; t.ldb[0] = wg.ld; t.planeB[0] = wg.plane;
+        t.B[1] = wu.p; t.ldb[1] = wu.ld; t.planeB[1] = wu.plane;
+        for (int q = 0; q < 2; ++q) { t.lda[q] = ldo; t.planeA[q] = plane; }
+        t.out_type = b.type; t.C[0] = b.dX; t.ldc[0] = b.lddx; t.ncols = out_cols(b.type, b.K, b.lddx);
+        if (const int rc = run_input_grad(ar, t, P, st)) return rc;
+    }
+    if (b.dW[0]) {
+        Planes x;
+        if (const int rc = make_planes(ar, b.X, b.M, b.K, PX, false, st, &x)) return rc;
+        TileArgs t = tile_args();
+        t.M = b.K; t.N = b.N; t.K[0] = b.M;
+        t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
+        t.B[0] = dG; t.B[1] = dU;
+        for (int q = 0; q < 2; ++q) { t.ldb[q] = ldo; t.planeB[q] = plane; t.C[q] = b.dW[q]; t.ldc[q] = b.lddw[q]; }
+        t.out_type = b.type;
+        t.ncols = std::max(out_cols(b.type, b.N, b.lddw[0]), out_cols(b.type, b.N, b.lddw[1]));
+        if (b.lddw[0] != b.lddw[1]) t.ncols = std::min(out_cols(b.type, b.N, b.lddw[0]), out_cols(b.type, b.N, b.lddw[1]));
+        if (const int rc = run_weight_grad(ar, t, PX, P, 2, st)) return rc;
+    }
+    return 0;
+}
+
+struct WgradArgs { int64_t M, K, N; int type, precision; MatIn X, dZ; void* dW; int64_t lddw; };
+int weight_grad_exact(Arena& ar, const WgradArgs& w, hipStream_t st) {
+    const int64_t ldx = up(w.K, 4);
+    float* x = static_cast<float*>(ar.take(w.M * ldx * 4));
+    const size_t need = geogcn_gemm_workspace_bytes(1, 0, w.K, w.N, w.M, GEOGCN_GEMM_F32);
+    void* g = ar.take((int64_t)need);
+    if (!ar.base) return 0;
+    if (const int rc = geogcn_mx8_unpack(w.M, (int32_t)w.K, GEOGCN_T_F32, static_cast<const uint8_t*>(w.X.p), w.X.ld, w.X.scale, x, ldx, st)) return rc;
+    return geogcn_gemm_f32(1, 0, w.K, w.N, w.M, x, ldx, static_cast<const float*>(w.dZ.p), w.dZ.ld, static_cast<float*>(w.dW), w.lddw, nullptr,
+                           GEOGCN_ACT_NONE, 0, GEOGCN_GEMM_F32, need ? g : nullptr, need, st);
+}
+int weight_grad(Arena& ar, const WgradArgs& w, hipStream_t st) {
+    if (w.precision == GEOGCN_GEMM_F32 && w.type == GEOGCN_T_F32) return weight_grad_exact(ar, w, st);
+    const int P = terms_of(w.type, w.precision);
+    Planes x, dz;
+    if (const int rc = make_planes(ar, w.X, w.M, w.K, 1, false, st, &x)) return rc;
+    if (const int rc = make_planes(ar, w.dZ, w.M, w.N, P, false, st, &dz)) return rc;
+    TileArgs t = tile_args();
+    t.M = w.K; t.N = w.N; t.K[0] = w.M;
+    t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
+    t.B[0] = dz.p; t.ldb[0] = dz.ld; t.planeB[0] = dz.plane;
+    t.C[0] = w.dW; t.ldc[0] = w.lddw; t.out_type = w.type; t.ncols = out_cols(w.type, w.N, w.lddw);
+    return run_weight_grad(ar, t, 1, P, 1, st);
+}
+
+// the pads of an fp32 matrix's quad lie inside its pitch (checked), so whole quads can be written; a zero-sized reduction gives zeros
+int zero_matrix(void* p, int type, int64_t n, int64_t cols, int64_t ld, hipStream_t st) {
+    if (type == GEOGCN_T_F32) return zero_rows_async(static_cast<float*>(p), n, cols, ld, st);
+    return zero_rows_async(static_cast<float*>(p), n, cols / 2, ld / 2, st);
+}
+
+int check_ws(const char* who, size_t need, const void* ws, size_t have) {
+    GEOGCN_REQUIRE(need == 0 || (ws && have >= need), GEOGCN_E_ARG, "%s: workspace of %zu bytes, %zu needed", who, have, need);
+    GEOGCN_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(ws) % 256 == 0, GEOGCN_E_ALIGN, "%s: workspace not on 256 bytes", who);
+    return 0;
+}
+
+}  // namespace
+}  // namespace geogcn
+
+using namespace geogcn;
+
+extern "C" int geogcn_gated_fwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx, const void* Wg, int64_t ldwg, const void* Wu,
+                                int64_t ldwu, const float* bg, const float* bu, int32_t act, void* H, int64_t ldh, int32_t keep, void* G, int64_t ldg,
+                                uint8_t* Gs, void* U, int64_t ldu, uint8_t* Us, int32_t precision, void* ws, size_t* ws_bytes, void* stream) {
+    const char* who = "gated_fwd";
+    if (const int rc = check_dims(who, M, K, N)) return rc;
+    GEOGCN_REQUIRE(ws_bytes, GEOGCN_E_NULL, "%s: ws_bytes is null", who);
+    GEOGCN_REQUIRE(type == GEOGCN_T_F32 || type == GEOGCN_T_BF16, GEOGCN_E_ARG, "%s: type %d is neither fp32 nor bf16", who, type);
+    GEOGCN_REQUIRE(precision >= GEOGCN_GEMM_F32 && precision <= GEOGCN_GEMM_BF16, GEOGCN_E_ARG, "%s: precision %d", who, precision);
+    GEOGCN_REQUIRE(act_ok(act), GEOGCN_E_ARG, "%s: activation %d", who, act);
+    GEOGCN_REQUIRE(keep == GEOGCN_KEEP_NONE || keep == GEOGCN_KEEP_FULL || keep == GEOGCN_KEEP_MX8, GEOGCN_E_ARG, "%s: keep %d", who, keep);
+    FwdArgs f;
+    f.M = M; f.K = K; f.N = N; f.type = type; f.precision = precision; f.keep = keep; f.act = act;
+    f.X = MatIn{type, X, ldx, nullptr}; f.Wg = MatIn{type, Wg, ldwg, nullptr}; f.Wu = MatIn{type, Wu, ldwu, nullptr};
+    f.bg = bg; f.bu = bu; f.H = H; f.ldh = ldh;
+    f.keepP[0] = G; f.keepP[1] = U; f.ldk[0] = ldg; f.ldk[1] = ldu; f.keepS[0] = Gs; f.keepS[1] = Us;
+    const bool empty = M == 0 || N == 0;
+    if (!empty) {
+        if (K > 0) {
+            if (const int rc = check_mat(who, "X", type, X, ldx, nullptr, K)) return rc;
+            if (const int rc = check_mat(who, "Wg", type, Wg, ldwg, nullptr, N)) return rc;
+            if (const int rc = check_mat(who, "Wu", type, Wu, ldwu, nullptr, N)) return rc;
+        }
+        if (const int rc = check_mat(who, "H", type, H, ldh, nullptr, N)) return rc;
+        if (keep != GEOGCN_KEEP_NONE) {
+            const int kt = keep == GEOGCN_KEEP_MX8 ? GEOGCN_T_MX8 : type;
+            if (const int rc = check_mat(who, "G", kt, G, ldg, Gs, N)) return rc;
+            if (const int rc = check_mat(who, "U", kt, U, ldu, Us, N)) return rc;
+            if (keep == GEOGCN_KEEP_FULL)
+                GEOGCN_REQUIRE(out_cols(type, N, ldg) >= out_cols(type, N, ldh) && out_cols(type, N, ldu) >= out_cols(type, N, ldh), GEOGCN_E_ALIGN,
+                               "%s: G and U need H's pitch", who);
+        }
+    }
+    Arena count{nullptr};
+    if (!empty) forward(count, f, nullptr);
+    if (!ws) {
+        *ws_bytes = std::max<size_t>(count.used, 256);
+        return 0;
+    }
+    if (empty) return 0;
+    if (const int rc = check_ws(who, count.used, ws, *ws_bytes)) return rc;
+    Arena ar{static_cast<unsigned char*>(ws)};
+    return forward(ar, f, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* dH, int64_t lddh, int32_t x_type, const void* X, int64_t ldx,
+                                const uint8_t* Xs, const void* Wg, int64_t ldwg, const void* Wu, int64_t ldwu, int32_t kept_type, const void* G,
+                                int64_t ldg, const uint8_t* Gs, const void* U, int64_t ldu, const uint8_t* Us, int32_t act, void* dX, int64_t lddx,
+                                void* dWg, int64_t lddwg, void* dWu, int64_t lddwu, float* dbg, float* dbu, int32_t precision, void* ws,
+                                size_t* ws_bytes, void* stream) {
+    const char* who = "gated_bwd";
+    if (const int rc = check_dims(who, M, K, N)) return rc;
+    GEOGCN_REQUIRE(ws_bytes, GEOGCN_E_NULL, "%s: ws_bytes is null", who);
+    GEOGCN_REQUIRE(type == GEOGCN_T_F32 || type == GEOGCN_T_BF16, GEOGCN_E_ARG, "%s: type %d is neither fp32 nor bf16", who, type);
+    GEOGCN_REQUIRE((x_type == type || x_type == GEOGCN_T_MX8) && (kept_type == type || kept_type == GEOGCN_T_MX8), GEOGCN_E_ARG,
+                   "%s: X and the kept G, U are of the block's type or 8-bit checkpoints (got %d, %d)", who, x_type, kept_type);
+    GEOGCN_REQUIRE(precision >= GEOGCN_GEMM_F32 && precision <= GEOGCN_GEMM_BF16, GEOGCN_E_ARG, "%s: precision %d", who, precision);
+    GEOGCN_REQUIRE(act_ok(act), GEOGCN_E_ARG, "%s: activation %d", who, act);
+    GEOGCN_REQUIRE((dWg == nullptr) == (dWu == nullptr) && (dbg == nullptr) == (dbu == nullptr), GEOGCN_E_NULL,
+                   "%s: the weight (bias) gradients come in pairs", who);
+    BwdArgs b;
+    b.M = M; b.K = K; b.N = N; b.type = type; b.precision = precision; b.act = act;
+    b.dH = MatIn{type, dH, lddh, nullptr}; b.X = MatIn{x_type, X, ldx, Xs}; b.G = MatIn{kept_type, G, ldg, Gs}; b.U = MatIn{kept_type, U, ldu, Us};
+    b.Wg = MatIn{type, Wg, ldwg, nullptr}; b.Wu = MatIn{type, Wu, ldwu, nullptr};
+    b.dX = dX; b.lddx = lddx; b.dW[0] = dWg; b.dW[1] = dWu; b.lddw[0] = lddwg; b.lddw[1] = lddwu; b.db[0] = dbg; b.db[1] = dbu;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (M > 0 && N > 0) {
+        if (const int rc = check_mat(who, "dH", type, dH, lddh, nullptr, N)) return rc;
+        if (const int rc = check_mat(who, "G", kept_type, G, ldg, Gs, N)) return rc;
+        if (const int rc = check_mat(who, "U", kept_type, U, ldu, Us, N)) return rc;
+        if (K > 0 && dX) {
+            if (const int rc = check_mat(who, "Wg", type, Wg, ldwg, nullptr, N)) return rc;
+            if (const int rc = check_mat(who, "Wu", type, Wu, ldwu, nullptr, N)) return rc;
+        }
+        if (K > 0 && dWg)
+            if (const int rc = check_mat(who, "X", x_type, X, ldx, Xs, K)) return rc;
+    }
+    if (dX && M > 0 && K > 0)
+        if (const int rc = check_mat(who, "dX", type, dX, lddx, nullptr, K)) return rc;
+    if (dWg && K > 0 && N > 0) {
+        if (const int rc = check_mat(who, "dWg", type, dWg, lddwg, nullptr, N)) return rc;
+        if (const int rc = check_mat(who, "dWu", type, dWu, lddwu, nullptr, N)) return rc;
+    }
+    if (dbg) GEOGCN_REQUIRE(aligned16(dbg) && aligned16(dbu), GEOGCN_E_ALIGN, "%s: bias gradients not aligned", who);
+    if (K == 0) { b.dX = nullptr; b.dW[0] = b.dW[1] = nullptr; }
+    const bool empty = M == 0 || N == 0;
+    Arena count{nullptr};
+    if (!empty) backward(count, b, nullptr);
+    if (!ws) {
+        *ws_bytes = std::max<size_t>(count.used, 256);
+        return 0;
+    }
+    if (empty) {                                             // no rows, or no units: sums over nothing
+        if (b.dX && M > 0)
+            if (const int rc = zero_matrix(dX, type, M, out_cols(type, K, lddx), lddx, st)) return rc;
+        for (int q = 0; q < 2; ++q) {
+            if (b.dW[q] && N > 0)
+                if (const int rc = zero_matrix(b.dW[q], type, K, out_cols(type, N, b.lddw[q]), b.lddw[q], st)) return rc;
+            if (b.db[q] && N > 0)
+                if (const int rc = zero_rows_async(b.db[q], 1, N, N, st)) return rc;
+        }
+        return 0;
+    }
+    if (const int rc = check_ws(who, count.used, ws, *ws_bytes)) return rc;
+    Arena ar{static_cast<unsigned char*>(ws)};
+    return backward(ar, b, st);
+}
+
+extern "C" int geogcn_mx8_weight_grad(int64_t M, int64_t K, int64_t N, int32_t type, const uint8_t* X, int64_t ldx, const uint8_t* Xs, const void* dZ,
+                                      int64_t lddz, void* dW, int64_t lddw, int32_t precision, void* ws, size_t* ws_bytes, void* stream) {
+    const char* who = "mx8_weight_grad";
+    if (const int rc = check_dims(who, M, K, N)) return rc;
+    GEOGCN_REQUIRE(ws_bytes, GEOGCN_E_NULL, "%s: ws_bytes is null", who);
+    GEOGCN_REQUIRE(type == GEOGCN_T_F32 || type == GEOGCN_T_BF16, GEOGCN_E_ARG, "%s: type %d is neither fp32 nor bf16", who, type);
+    GEOGCN_REQUIRE(precision >= GEOGCN_GEMM_F32 && precision <= GEOGCN_GEMM_BF16, GEOGCN_E_ARG, "%s: precision %d", who, precision);
+    const bool none = K == 0 || N == 0;
+    if (!none) {
+        if (const int rc = check_mat(who, "dW", type, dW, lddw, nullptr, N)) return rc;
+        if (M > 0) {
+            if (const int rc = check_mat(who, "X", GEOGCN_T_MX8, X, ldx, Xs, K)) return rc;
+            if (const int rc = check_mat(who, "dZ", type, dZ, lddz, nullptr, N)) return rc;
+        }
+    }
+    WgradArgs w{M, K, N, type, precision, MatIn{GEOGCN_T_MX8, X, ldx, Xs}, MatIn{type, dZ, lddz, nullptr}, dW, lddw};
+    Arena count{nullptr};
+    if (!none && M > 0) weight_grad(count, w, nullptr);
+    if (!ws) {
+        *ws_bytes = std::max<size_t>(count.used, 256);
+        return 0;
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (none) return 0;
+    if (M == 0) return zero_matrix(dW, type, K, out_cols(type, N, lddw), lddw, st);
+    if (const int rc = check_ws(who, count.used, ws, *ws_bytes)) return rc;
+    Arena ar{static_cast<unsigned char*>(ws)};
+    return weight_grad(ar, w, st);
+}

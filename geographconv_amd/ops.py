@@ -12,7 +12,7 @@ import scipy.sparse as sps
 import torch
 
 from . import _ffi, tuning
-from ._ffi import ACT_NONE, ACT_RELU, ACT_SELU, ACT_SIGMOID, ACT_TANH, check  # noqa: F401
+from ._ffi import ACT_GELU, ACT_NONE, ACT_RELU, ACT_SELU, ACT_SIGMOID, ACT_SILU, ACT_TANH, check  # noqa: F401
 
 
 class StepTimers:
@@ -1163,3 +1163,249 @@ class SpmmTimer:
                 self._h = C.c_void_p(0)
         except Exception:
             pass
+
+
+# --------------------------------------------------------------------------------------------
+# 8-bit activation checkpoints and the gated dense block (include/geogcn.h geogcn_mx8_*, geogcn_gated_*)
+# --------------------------------------------------------------------------------------------
+class MX8Mat:
+    """A matrix kept in 8 bits: e4m3 `codes` [n, roundup32(F)] and one power-of-two `scales` byte per 32 consecutive values of a row
+    (1.03 bytes a value).  `bf16`: what it was written from and reads back as (an HMat; else a DMat)."""
+    __slots__ = ('codes', 'scales', 'n', 'F', 'bf16')
+
+    def __init__(self, n, F, codes, scales, bf16=False):
+        self.n, self.F, self.bf16 = int(n), int(F), bool(bf16)
+        w = (self.F + 31) // 32
+        for t, what in ((codes, 'codes'), (scales, 'scales')):
+            if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_contiguous() or t.shape[0] != self.n:
+                raise ValueError("MX8Mat: %s must be a contiguous uint8 matrix of %d rows" % (what, self.n))
+        if codes.shape[1] < 32 * w or codes.shape[1] != 32 * scales.shape[1]:
+            raise ValueError("MX8Mat: %d columns need whole blocks of 32 codes and a scale for each, got %s and %s"
+                             % (self.F, tuple(codes.shape), tuple(scales.shape)))
+        if scales.device != codes.device:
+            raise ValueError("MX8Mat: codes and scales live on different devices")
+        self.codes, self.scales = codes, scales
+
+    @staticmethod
+    def empty(n, F, device, bf16=False):
+        w = (int(F) + 31) // 32
+        return MX8Mat(n, F, torch.empty((int(n), 32 * w), dtype=torch.uint8, device=device),
+                      torch.empty((int(n), w), dtype=torch.uint8, device=device), bf16)
+
+    @property
+    def ld(self):
+        return self.codes.shape[1]
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def numpy(self):
+        return mx8_unpack(self).numpy()
+
+
+class GatedTape:
+    """What a gated block's forward kept for its backward: G = X.Wg + bg and U = X.Wu + bu, both DMat / HMat or both MX8Mat."""
+    __slots__ = ('G', 'U')
+
+    def __init__(self, G, U):
+        if type(G) is not type(U) or (G.n, G.F) != (U.n, U.F):
+            raise ValueError("GatedTape: G and U must be of one kind and shape")
+        self.G, self.U = G, U
+
+
+def _mat_type(m):
+    if isinstance(m, MX8Mat):
+        return _ffi.T_MX8
+    if isinstance(m, HMat):
+        return _ffi.T_BF16
+    if isinstance(m, DMat):
+        return _ffi.T_F32
+    raise ValueError("expected a DMat, HMat or MX8Mat, got %s" % type(m).__name__)
+
+
+def _mat_args(m):
+    """(pointer, pitch) of a dense matrix, (codes, pitch, scales) where a checkpoint may stand too"""
+    return (_p(m.codes), m.ld, _p(m.scales)) if isinstance(m, MX8Mat) else (_p(m.t), m.ld, C.c_void_p(0))
+
+
+def _new_like_block(bf16, n, F, device):
+    return HMat(n, F, device) if bf16 else DMat.empty(n, F, device)
+
+
+def _same_device(*ms):
+    dev = ms[0].device
+    if any(m is not None and m.device != dev for m in ms):
+        raise ValueError("operands live on different devices: %s" % sorted({str(m.device) for m in ms if m is not None}))
+    if dev.type != 'cuda':
+        raise _ffi.GeoGcnError("operands live on %s: there is no CPU path" % dev)
+    return dev
+
+
+def _check_out(m, n, F, kind, what):
+    if not isinstance(m, kind) or m.n != n or m.F != F:
+        raise ValueError("%s must be a %s of %d x %d" % (what, kind.__name__, n, F))
+    return m
+
+
+def _check_vec(v, N, what):
+    if v is not None and (v.dtype != torch.float32 or v.dim() != 1 or not v.is_contiguous() or v.numel() < N):
+        raise ValueError("%s must be a contiguous fp32 vector of at least %d values" % (what, N))
+    return v
+
+
+def _run_with_ws(fn, name, args, dev):
+    """Ask the entry point for its scratch, allocate it for this call alone (stream-ordered; a captured call's lives in the graph's
+    pool, so two graphs never share one) and launch on the current stream of the operands' device."""
+    with torch.cuda.device(dev):
+        need = C.c_size_t(0)
+        check(fn(*args, C.c_void_p(0), C.byref(need), C.c_void_p(0)), name)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        check(fn(*args, _p(ws), C.byref(need), _stream()), name)
+
+
+@_timed('mx8_pack')
+def mx8_pack(X, out: MX8Mat = None):
+    """X (DMat or HMat) kept in 8 bits: blocks of 32 values of a row share the smallest power-of-two scale that saturates none of them;
+    every value is off by at most 2^-4 of itself (or 2^-10 of the scale)."""
+    t = _mat_type(X)
+    if t == _ffi.T_MX8:
+        raise ValueError("mx8_pack: already an 8-bit checkpoint")
+    bf16 = t == _ffi.T_BF16
+    if out is None:
+        out = MX8Mat.empty(X.n, X.F, X.device, bf16)
+    elif (out.n, out.F, out.bf16) != (X.n, X.F, bf16):
+        raise ValueError("mx8_pack: the output does not have the input's shape and type")
+    dev = _same_device(X, out)
+    with torch.cuda.device(dev):
+        check(_ffi.lib().geogcn_mx8_pack(X.n, X.F, t, _p(X.t), X.ld, _p(out.codes), out.ld, _p(out.scales), _stream()), 'mx8_pack')
+    return out
+
+
+@_timed('mx8_unpack')
+def mx8_unpack(Q: MX8Mat, out=None):
+    """The values a checkpoint stands for, as a DMat (HMat where it was written from one); pad columns zero."""
+    if _mat_type(Q) != _ffi.T_MX8:
+        raise ValueError("mx8_unpack: not an 8-bit checkpoint")
+    kind = HMat if Q.bf16 else DMat
+    out = _new_like_block(Q.bf16, Q.n, Q.F, Q.device) if out is None else _check_out(out, Q.n, Q.F, kind, 'mx8_unpack: the output')
+    dev = _same_device(Q, out)
+    with torch.cuda.device(dev):
+        check(_ffi.lib().geogcn_mx8_unpack(Q.n, Q.F, _mat_type(out), _p(Q.codes), Q.ld, _p(Q.scales), _p(out.t), out.ld, _stream()), 'mx8_unpack')
+    return out
+
+
+@_timed('mx8_weight_grad')
+def mx8_weight_grad(X: MX8Mat, dZ, out=None, precision=None):
+    """X^T . dZ with X kept in 8 bits: the weight gradient of a dense layer from its checkpointed input.  `precision`: 'bf16x3'
+    (fp32-class), 'bf16', or 'f32' (the checkpoint is read back and the exact fp32 kernel multiplies)."""
+    if _mat_type(X) != _ffi.T_MX8 or _mat_type(dZ) == _ffi.T_MX8:
+        raise ValueError("mx8_weight_grad takes an 8-bit checkpoint and a dense gradient")
+    bf16 = isinstance(dZ, HMat)
+    if dZ.n != X.n or X.bf16 != bf16:
+        raise ValueError("mx8_weight_grad: the checkpoint (%d rows, %s) and dZ (%d rows, %s) do not match"
+                         % (X.n, 'bf16' if X.bf16 else 'fp32', dZ.n, 'bf16' if bf16 else 'fp32'))
+    prec = _block_precision(precision, bf16)
+    out = _new_like_block(bf16, X.F, dZ.F, X.device) if out is None else _check_out(out, X.F, dZ.F, HMat if bf16 else DMat, 'mx8_weight_grad: the output')
+    dev = _same_device(X, dZ, out)
+    _run_with_ws(_ffi.lib().geogcn_mx8_weight_grad, 'mx8_weight_grad',
+                 (X.n, X.F, dZ.F, _mat_type(dZ), *_mat_args(X), _p(dZ.t), dZ.ld, _p(out.t), out.ld, prec), dev)
+    return out
+
+
+GATED_ACTS = (ACT_NONE, ACT_TANH, ACT_SIGMOID, ACT_RELU, ACT_SILU, ACT_GELU)
+
+
+def _block_precision(precision, bf16):
+    """-> GEMM_* of the block's products: a bf16 block has one kind; an fp32 one follows `precision` (None: the default)."""
+    p = precision or GEMM_PRECISION
+    if p not in GEMM_PRECISIONS:
+        raise ValueError("unknown precision %r" % (precision,))
+    return _ffi.GEMM_BF16 if bf16 else GEMM_PRECISIONS[p]
+
+
+def _check_gated(X, Wg, Wu, act, who):
+    """-> (bf16 block?, rows, inputs, units)"""
+    if act not in GATED_ACTS:
+        raise ValueError("%s: activation %r is not one of %r" % (who, act, GATED_ACTS))
+    tw = _mat_type(Wg)
+    if tw == _ffi.T_MX8 or _mat_type(Wu) != tw:
+        raise ValueError("%s: both weights must be DMat or both HMat" % who)
+    bf16 = tw == _ffi.T_BF16
+    if (X.bf16 if isinstance(X, MX8Mat) else isinstance(X, HMat)) != bf16:
+        raise ValueError("%s: the input and the weights are of different types" % who)
+    if (Wu.n, Wu.F) != (Wg.n, Wg.F) or Wg.n != X.F:
+        raise ValueError("%s: input %d x %d, weights %d x %d and %d x %d" % (who, X.n, X.F, Wg.n, Wg.F, Wu.n, Wu.F))
+    return bf16, X.n, X.F, Wg.F
+
+
+@_timed('gated_dense')
+def gated_dense(X, Wg, Wu, bg: torch.Tensor = None, bu: torch.Tensor = None, act=ACT_SIGMOID, out=None, keep=None, precision=None):
+    """act(X . Wg + bg) * (X . Wu + bu), both projections, the activation and the product in one kernel.  All matrices DMat, or all
+    HMat (bf16 storage, fp32 accumulation; biases stay fp32).  `keep`: None -> the result alone; 'full' / 'mx8' -> (result, GatedTape) with
+    G and U kept in the block's type / in 8 bits for gated_dense_bwd.  `precision` (fp32 block): 'bf16x3', 'bf16', or 'f32' -- the exact
+    fp32 products, in their own launches."""
+    if keep not in (None, 'full', 'mx8'):
+        raise ValueError("gated_dense: keep is None, 'full' or 'mx8', not %r" % (keep,))
+    if isinstance(X, MX8Mat):
+        raise ValueError("gated_dense: the input must be dense")
+    bf16, M, K, N = _check_gated(X, Wg, Wu, act, 'gated_dense')
+    _check_vec(bg, N, 'gated_dense: bg')
+    _check_vec(bu, N, 'gated_dense: bu')
+    prec = _block_precision(precision, bf16)
+    kind = HMat if bf16 else DMat
+    H = _new_like_block(bf16, M, N, X.device) if out is None else _check_out(out, M, N, kind, 'gated_dense: the output')
+    dev = _same_device(X, Wg, Wu, bg, bu, H)
+    lib = _ffi.lib()
+    G = U = None
+    if keep == 'full':
+        G, U = (HMat(M, N, dev, ld=H.ld) if bf16 else DMat.empty(M, N, dev, ld=H.ld) for _ in range(2))
+    elif keep == 'mx8':
+        G, U = MX8Mat.empty(M, N, dev, bf16), MX8Mat.empty(M, N, dev, bf16)
+    none = (C.c_void_p(0), 0, C.c_void_p(0))
+    _run_with_ws(lib.geogcn_gated_fwd, 'gated_fwd',
+                 (M, K, N, _mat_type(X), _p(X.t), X.ld, _p(Wg.t), Wg.ld, _p(Wu.t), Wu.ld, _p(bg), _p(bu), int(act), _p(H.t), H.ld,
+                  {None: _ffi.KEEP_NONE, 'full': _ffi.KEEP_FULL, 'mx8': _ffi.KEEP_MX8}[keep], *(_mat_args(G) if keep else none),
+                  *(_mat_args(U) if keep else none), prec), dev)
+    return H if keep is None else (H, GatedTape(G, U))
+
+
+@_timed('gated_dense_bwd')
+def gated_dense_bwd(dH, X, Wg, Wu, kept: GatedTape, act=ACT_SIGMOID, dX=None, dWg=None, dWu=None, dbg: torch.Tensor = None,
+                    dbu: torch.Tensor = None, bias=False, need_input_grad=True, precision=None):
+    """-> (dX, dWg, dWu, dbg, dbu) of gated_dense from the gradient dH of its result, its input X and the kept G, U -- X and `kept` each
+    dense or in 8 bits (MX8Mat).  The gradient buffers may be given; `bias` (or a given dbg / dbu pair) asks for the bias gradients,
+    `need_input_grad=False` leaves dX out (None comes back).  `act` and `precision` must be the forward's."""
+    bf16, M, K, N = _check_gated(X, Wg, Wu, act, 'gated_dense_bwd')
+    kind = HMat if bf16 else DMat
+    _check_out(dH, M, N, kind, 'gated_dense_bwd: dH')
+    tk = _mat_type(kept.G)
+    if (kept.G.n, kept.G.F) != (M, N) or (kept.G.bf16 or kept.U.bf16 if tk == _ffi.T_MX8 else isinstance(kept.G, HMat)) != bf16:
+        raise ValueError("gated_dense_bwd: the kept G, U are not those of a %d x %d block of this type" % (M, N))
+    if (dbg is None) != (dbu is None) or (dWg is None) != (dWu is None):
+        raise ValueError("gated_dense_bwd: gradient buffers of the two branches come in pairs")
+    for m, n, F, what in ((dX, M, K, 'dX'), (dWg, K, N, 'dWg'), (dWu, K, N, 'dWu')):
+        if m is not None:
+            _check_out(m, n, F, kind, 'gated_dense_bwd: ' + what)
+    prec = _block_precision(precision, bf16)
+    dev = _same_device(dH, X, Wg, Wu, kept.G, kept.U, dX, dWg, dWu, dbg, dbu)
+    bias = bias or dbg is not None
+    if bias and dbg is None:
+        dbg, dbu = (torch.zeros(pad4(N), dtype=torch.float32, device=dev) for _ in range(2))
+    for v, what in ((dbg, 'dbg'), (dbu, 'dbu')):
+        _check_vec(v, pad4(N) if bias else 0, 'gated_dense_bwd: ' + what)
+    if need_input_grad:
+        dX = _new_like_block(bf16, M, K, dev) if dX is None else dX
+    else:
+        dX = None
+    if dWg is None:
+        dWg, dWu = (_new_like_block(bf16, K, N, dev) for _ in range(2))
+    _run_with_ws(_ffi.lib().geogcn_gated_bwd, 'gated_bwd',
+                 (M, K, N, _mat_type(dH), _p(dH.t), dH.ld, _mat_type(X), *_mat_args(X), _p(Wg.t), Wg.ld, _p(Wu.t), Wu.ld, tk,
+                  *_mat_args(kept.G), *_mat_args(kept.U), int(act), _p(dX.t if dX is not None else None), dX.ld if dX is not None else 0,
+                  _p(dWg.t), dWg.ld, _p(dWu.t), dWu.ld, _p(dbg), _p(dbu), prec), dev)
+    return dX, dWg, dWu, dbg, dbu

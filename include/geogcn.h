@@ -52,6 +52,14 @@ extern "C" {
 /* elementwise entry points only (geogcn_bias_act_f32 / geogcn_act_bwd_f32), not fused epilogues: */
 #define GEOGCN_ACT_SELU    3   /* lasagne.nonlinearities.selu     gcnmodel.py:290 (residual_dense) */
 #define GEOGCN_ACT_RELU    4   /* lasagne.nonlinearities.rectify  gcnmodel.py:345 (commented out)  */
+/* the gated dense block only (geogcn_gated_*), beside NONE, TANH, SIGMOID and RELU: */
+#define GEOGCN_ACT_SILU    5   /* x * sigmoid(x)                                                   */
+#define GEOGCN_ACT_GELU    6   /* x * Phi(x), Phi the normal distribution's (no approximation)     */
+
+/* storage types of the matrices that the gated block and the 8-bit checkpoints take */
+#define GEOGCN_T_F32  0
+#define GEOGCN_T_BF16 1        /* pads of a row zero up to roundup64(cols) or the pitch, whichever is less */
+#define GEOGCN_T_MX8  2        /* e4m3 codes, one byte a value, + one scale byte per 32 (geogcn_mx8_pack)  */
 
 int         geogcn_version(void);
 const char* geogcn_last_error(void);
@@ -484,6 +492,45 @@ int geogcn_adam_step_ctr_f32(int64_t n, float* p, float* g, float* m, float* v, 
 /* penalty value: sum regmask*(l1*|p| + l2*p^2) -> out[0] (deterministic two-pass)               */
 int geogcn_reg_penalty_f32(int64_t n, const float* p, const float* regmask, float l1, float l2,
                            float* out, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- 8-bit activation checkpoints (no reference counterpart: the reference keeps fp32 activations) -------------------------------
+ * A row's values are taken in blocks of 32 that share a scale 2^s, s the smallest exponent (-126 at least) with max|x| <= 448 * 2^s, stored as
+ * the byte s + 127 in scale[n x ldq / 32]; codes[n x ldq] holds e4m3 codes of x / 2^s, round to nearest even (codes behind column F are 0).
+ * No value saturates.  A block with an infinity or a NaN has the scale byte 255 and reads back as NaN throughout.  type: that of X / Y
+ * (GEOGCN_T_F32 or GEOGCN_T_BF16).  ldx % 4 == 0, ldq % 32 == 0, ldq >= F; X / Y aligned to 16 (fp32) / 8 (bf16) bytes, codes to 4.
+ * unpack writes the pad columns of Y (roundup4 / roundup64, never past the pitch) as zero.                                                */
+int geogcn_mx8_pack(int64_t n, int32_t F, int32_t type, const void* X, int64_t ldx, uint8_t* codes, int64_t ldq, uint8_t* scale, void* stream);
+int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, int64_t ldq, const uint8_t* scale, void* Y, int64_t ldy,
+                      void* stream);
+
+/* ---- the gated dense block: H = act(X.Wg + bg) * (X.Wu + bu), X [M x K], W [K x N] (no reference counterpart; sibling of the highway
+ * block, gcnmodel.py:268-288) -------------------------------------------------------------------------------------------------------------
+ * type: GEOGCN_T_F32 or GEOGCN_T_BF16, that of every matrix; bg, bu: fp32, may be NULL (each on its own).  Products of fp32 matrices:
+ * GEOGCN_GEMM_F32 (the exact fp32 kernels, in launches of their own), GEOGCN_GEMM_BF16X3 (three bf16 terms a value, fp32-class) or
+ * GEOGCN_GEMM_BF16 (operands rounded to bf16); accumulation fp32.  (An infinity is not the sum of three bf16 terms: under BF16X3 its row
+ * gives NaN.)  Products of bf16 matrices are one kind, whatever `precision` says.
+ * keep: what of G = X.Wg + bg and U = X.Wu + bu is stored for the backward -- nothing, in the block's type (pitch >= H's), or as 8-bit
+ * checkpoints (codes G / U with pitch ldg / ldu and scales Gs / Us as geogcn_mx8_pack writes them).
+ * ws: scratch.  Call with ws = NULL to have *ws_bytes set to what the call needs (no launch); then with ws (256-byte aligned) and its size.
+ * How operands are read depends on their addresses: ask with the very arguments of the call.  Nothing in ws outlives the call.            */
+#define GEOGCN_KEEP_NONE 0
+#define GEOGCN_KEEP_FULL 1
+#define GEOGCN_KEEP_MX8  2
+int geogcn_gated_fwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx, const void* Wg, int64_t ldwg, const void* Wu,
+                     int64_t ldwu, const float* bg, const float* bu, int32_t act, void* H, int64_t ldh, int32_t keep, void* G, int64_t ldg,
+                     uint8_t* Gs, void* U, int64_t ldu, uint8_t* Us, int32_t precision, void* ws, size_t* ws_bytes, void* stream);
+/* Its backward from dH, X and the kept G, U (x_type / kept_type: the block's type or GEOGCN_T_MX8 with scales Xs / Gs, Us):
+ *   dG = dH * U * act'(G), dU = dH * act(G);  dX = dG.Wg^T + dU.Wu^T;  dWg = X^T.dG, dWu = X^T.dU;  dbg, dbu = column sums (fp32).
+ * dX, the pair dWg / dWu and the pair dbg / dbu may each be NULL (not formed).  In a bf16 block dG and dU are rounded to bf16 before the
+ * products, not before the bias gradients.  ws: as above.                                                                                 */
+int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* dH, int64_t lddh, int32_t x_type, const void* X, int64_t ldx,
+                     const uint8_t* Xs, const void* Wg, int64_t ldwg, const void* Wu, int64_t ldwu, int32_t kept_type, const void* G, int64_t ldg,
+                     const uint8_t* Gs, const void* U, int64_t ldu, const uint8_t* Us, int32_t act, void* dX, int64_t lddx, void* dWg,
+                     int64_t lddwg, void* dWu, int64_t lddwu, float* dbg, float* dbu, int32_t precision, void* ws, size_t* ws_bytes, void* stream);
+/* dW [K x N] = X^T.dZ of a dense layer whose input X [M x K] was kept as an 8-bit checkpoint (type: that of dZ and dW).  A checkpointed value is
+ * one bf16 term: three cross products a value of fp32 dZ instead of six.  ws: as above.                                                    */
+int geogcn_mx8_weight_grad(int64_t M, int64_t K, int64_t N, int32_t type, const uint8_t* X, int64_t ldx, const uint8_t* Xs, const void* dZ,
+                           int64_t lddz, void* dW, int64_t lddw, int32_t precision, void* ws, size_t* ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
