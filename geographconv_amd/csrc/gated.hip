@@ -8,7 +8,7 @@
 // All three products run on ONE tiled kernel over bf16 TERMS: an fp32 value is the exact sum of three bf16 values, and a product of two
 // fp32 matrices is the sum of its six largest cross products (the dropped ones are O(2^-24)), accumulated in fp32; a bf16 value is one term
 // and so is an 8-bit checkpoint's (4 significant bits), so X^T.dG from a checkpoint costs three cross products instead of six and loses
-// nothing on the way.  fp32 (and 8-bit) operands are written as term planes [term][row][roundup64(cols)] by terms_kernel or by the pass
+// nothing on the way.  fp32 (and 8-bit) operands are written as terms side by side, [row][term][roundup64(cols)], by terms_kernel or by the pass
 // that forms them; bf16 matrices whose rows are 16-byte aligned are read in place.
 #include "mx8.h"
 
@@ -108,14 +108,6 @@ struct TileArgs {
 };
 enum { EPI_STORE = 0, EPI_SLAB = 1, EPI_GATED = 2 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, int64_t bytes) {
-    const uint32_t n = bytes <= 0 ? 0u : (bytes > 0x7FFFFFFFll ? 0x7FFFFFFFu : (uint32_t)bytes);
-    const uint64_t b = reinterpret_cast<uint64_t>(base);
-    const uint64_t bu = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
-                        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(bu), 0, __builtin_amdgcn_readfirstlane(n), 0x00020000);
-}
-
 __device__ __forceinline__ void store_quad(void* C, int64_t ld, int type, int64_t row, int64_t col, const float (&x)[4]) {
     if (type == GEOGCN_T_F32)
         *reinterpret_cast<float4*>(static_cast<float*>(C) + row * ld + col) = make_float4(x[0], x[1], x[2], x[3]);
@@ -154,12 +146,13 @@ struct Image {
             return c < 0 ? c + kCpr : c;
         }
     }
-    // byte offset, from the image's first row and k, of the piece that belongs at place `piece` of the image (kOob: nothing there)
-    static __device__ __forceinline__ uint32_t source(int piece, int64_t ld, int64_t k_left) {
+    // byte offset, from the image's first row and k, of the piece that belongs at place `piece` of the image
+    static __device__ __forceinline__ uint32_t source(int piece, int64_t ld) {
         const int row = piece / kCpr, c = unplace(piece - row * kCpr, row);
-        if constexpr (STRIDED) return (uint32_t)row * (uint32_t)(ld * 2) + (uint32_t)c * 16u;      // (rows behind the last k: past the descriptor's end)
-        else return c * 8 < k_left ? (uint32_t)row * (uint32_t)(ld * 2) + (uint32_t)c * 16u : kOob;
+        return (uint32_t)row * (uint32_t)(ld * 2) + (uint32_t)c * 16u;
     }
+    // k-contiguous: the first of the 8 k-values of a lane's piece -- the same in every wave load (64 pieces are whole rows, and whole rounds of `place`)
+    static __device__ __forceinline__ int k_of_lane(int lane) { return unplace(lane % kCpr, lane / kCpr) * 8; }
     // the fragment of 16 rows from r0: lane (li, lg) gets its row's k-values s*32 + lg*8 .. + 7
     static __device__ __forceinline__ bf16x8 read(const unsigned char* img, int r0, int s, int li, int lg) {
         if constexpr (!STRIDED) {
@@ -176,7 +169,35 @@ struct Image {
     }
 };
 
-template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, bool GATED>
+// 64 lanes x 16 bytes from global memory to LDS (lane i's to lds + 16 i).  As assembly, so that the compiler, which cannot tell the buffer being
+// filled from the one being read, does not wait for these loads at every LDS read: the waits stand at the stage's barrier (stage_barrier).  M0 is
+// set and used inside the statement; nothing else in these kernels uses it.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+// all but the newest `LEFT` of this wave's loads have landed, its LDS reads are done, and so they are in every wave of the block
+template <int LEFT>
+__device__ __forceinline__ void stage_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(LEFT) : "memory");
+}
+// where an operand is read: the address of its first row and k of the stage, and the bytes from there to the matrix' end (reads behind: zeros)
+struct Cursor {
+    uint64_t p;
+    int64_t left;
+    __device__ __forceinline__ void set(const uint16_t* base, int64_t offset, int64_t total) {
+        p = reinterpret_cast<uint64_t>(base) + (uint64_t)offset * 2;
+        left = (total - offset) * 2;
+    }
+    __device__ __forceinline__ void advance(int64_t bytes) { p += (uint64_t)bytes; left -= bytes; }
+    __device__ __forceinline__ i32x4 rsrc() const {
+        const int n = left <= 0 ? 0 : left > 0x7FFFFFFFll ? 0x7FFFFFFF : (int)left;
+        return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)p), __builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32)),
+                     __builtin_amdgcn_readfirstlane(n), 0x00020000};
+    }
+};
+
+template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, int ST, bool GATED>
 __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
     constexpr int NW = WM * WN;
     constexpr int BNS = BN / NSEG;                            // columns of a segment
@@ -186,7 +207,9 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
     constexpr int CW = BNS / WN, NTS = CW / 16, NT = NTS * NSEG;
     static_assert(BM % (WM * 16) == 0 && CW % 16 == 0 && (!GATED || (NSEG == 2 && CW % 32 == 0)), "wave tiles");
     constexpr int kA = PA * IA::kBytes, kStage = kA + PB * NSEG * IB::kBytes;
-    constexpr int LA = PA * IA::kPieces / 64, LB = PB * NSEG * IB::kPieces / 64, LOADS = LA + LB;      // wave loads of a stage
+    constexpr int LIA = IA::kPieces / 64, LIB = IB::kPieces / 64;                   // wave loads of an image
+    constexpr int LA = PA * LIA / NW, LB = PB * NSEG * LIB / NW;                    // ... of a stage, per wave
+    static_assert(PA * LIA % NW == 0 && PB * LIB % NW == 0, "every wave loads as much of each operand");
     extern __shared__ __attribute__((aligned(128))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wid / WN, wn = wid % WN;
@@ -214,44 +237,80 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto issue = [&](int t, int buf) __attribute__((always_inline)) {
-        const int ks = t >= ns0 ? 1 : 0;
-        const int64_t k0 = (int64_t)(ks ? t - ns0 : t) * BK, Kl = (ks ? a.K[1] : a.K[0]) - k0;
-        const int64_t lda = ks ? a.lda[1] : a.lda[0], ldb0 = ks ? a.ldb[1] : a.ldb[0];
+    // this wave's loads of a stage: LA pieces of A's images, then LB of B's (segment by segment), 64 x 16 bytes each
+    uint32_t va[LA], vb[LB];
+    const int ka = IA::k_of_lane(lane), kb = IB::k_of_lane(lane);
+    Cursor ca, cb[NSEG];
+    int64_t k_left;
+    auto start = [&](int ks, int step) __attribute__((always_inline)) {      // cursors at stage `step` of reduction segment ks
+        const int64_t k0 = (int64_t)step * BK, K = a.K[ks];
+        const int64_t lda = a.lda[ks];
+        k_left = K - k0;
+        if constexpr (ASTR) ca.set(a.A[ks], k0 * lda + m0, K * lda);
+        else ca.set(a.A[ks], m0 * lda + k0, a.M * lda);
 #pragma unroll
-        for (int i = 0; i < (LOADS + NW - 1) / NW; ++i) {
-            const int l = i * NW + wid;
-            if (LOADS % NW != 0 && l >= LOADS) break;
-            const bool isA = LB == 0 || l < LA;
-            const uint16_t* base;
-            int64_t left;                                     // elements from `base` to the end of the plane
-            uint32_t voff;
-            if (isA) {
-                const int p = l / (IA::kPieces / 64), sub = l - p * (IA::kPieces / 64);
-                base = (ks ? a.A[1] : a.A[0]) + p * (ks ? a.planeA[1] : a.planeA[0]);
-                if constexpr (ASTR) { base += k0 * lda + m0; left = Kl * lda - m0; }
-                else { base += m0 * lda + k0; left = (a.M - m0) * lda - k0; }
-                voff = IA::source(sub * 64 + lane, lda, Kl);
-            } else {
-                const int lb = l - LA;
-                const int img = lb / (IB::kPieces / 64), sub = lb - img * (IB::kPieces / 64), sg = NSEG == 2 ? img / PB : 0, p = img - sg * PB;
-                const int w = NSEG == 2 ? sg : ks;
-                const int64_t ldb = NSEG == 2 ? (sg ? a.ldb[1] : a.ldb[0]) : ldb0;
-                base = (w ? a.B[1] : a.B[0]) + p * (w ? a.planeB[1] : a.planeB[0]);
-                if constexpr (BSTR) { base += k0 * ldb + n0; left = Kl * ldb - n0; }
-                else { base += n0 * ldb + k0; left = (a.N - n0) * ldb - k0; }
-                voff = IB::source(sub * 64 + lane, ldb, Kl);
-            }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(base, left * 2), (__attribute__((address_space(3))) void*)(lds + buf * kStage + l * 1024),
-                                                     16, (int)voff, 0, 0, 0);
+        for (int q = 0; q < NSEG; ++q) {
+            const int w = NSEG == 2 ? q : ks;
+            const int64_t ldb = a.ldb[w];
+            if constexpr (BSTR) cb[q].set(a.B[w], k0 * ldb + n0, K * ldb);
+            else cb[q].set(a.B[w], n0 * ldb + k0, a.N * ldb);
+        }
+#pragma unroll
+        for (int i = 0; i < LA; ++i) {
+            const int l = i * NW + wid, p = l / LIA;
+            va[i] = IA::source((l - p * LIA) * 64 + lane, lda) + (uint32_t)(p * a.planeA[ks] * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < LB; ++i) {
+            const int l = i % (LB / NSEG) * NW + wid, p = l / LIB;
+            vb[i] = IB::source((l - p * LIB) * 64 + lane, a.ldb[NSEG == 2 ? i / (LB / NSEG) : ks]) + (uint32_t)(p * a.planeB[NSEG == 2 ? 0 : ks] * 2);
         }
     };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + (uint32_t)wid * 1024u;
+    int next = t0, fill = 0;                                  // the stage to load next, and the buffer that it goes to
+    auto issue = [&]() __attribute__((always_inline)) {
+        if (a.n_kseg == 2 && next == ns0) start(1, 0);
+        const i32x4 ra = ca.rsrc();
+        i32x4 rb[NSEG];
+#pragma unroll
+        for (int q = 0; q < NSEG; ++q) rb[q] = cb[q].rsrc();
+        const uint32_t to = lds0 + (uint32_t)(fill * kStage);
+        const bool tail = k_left < BK;                        // (k-strided rows behind the last are behind the matrix' end; k-contiguous ones are not)
+#pragma unroll
+        for (int i = 0; i < LA; ++i) {
+            uint32_t v = va[i];
+            if (!ASTR && tail) v = ka < k_left ? v : kOob;
+            load_to_lds(ra, v, to + (uint32_t)(i * NW * 1024));
+        }
+#pragma unroll
+        for (int i = 0; i < LB; ++i) {
+            uint32_t v = vb[i];
+            if (!BSTR && tail) v = kb < k_left ? v : kOob;
+            load_to_lds(rb[i / (LB / NSEG)], v, to + (uint32_t)(kA + i * NW * 1024));
+        }
+        const int ks = a.n_kseg == 2 && next >= ns0 ? 1 : 0;
+        ca.advance(ASTR ? (int64_t)BK * 2 * a.lda[ks] : BK * 2);
+#pragma unroll
+        for (int q = 0; q < NSEG; ++q) cb[q].advance(BSTR ? (int64_t)BK * 2 * a.ldb[NSEG == 2 ? q : ks] : BK * 2);
+        k_left -= BK;
+        ++next;
+        fill = fill + 1 == ST ? 0 : fill + 1;
+    };
 
-    if (t0 < t1) issue(t0, 0);
+    if (t0 < t1) {
+        if (a.n_kseg == 2 && t0 > ns0) start(1, t0 - ns0);
+        else start(0, t0);                                    // (t0 == ns0: issue() starts the second segment)
+    }
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i)
+        if (t0 + i < t1) issue();
+    int buf = 0;
+#pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        __syncthreads();                                      // stage t has landed, and nobody reads the other buffer any more
-        if (t + 1 < t1) issue(t + 1, buf ^ 1);
+        // stage t has landed, and nobody reads the buffer of stage t - 1 any more
+        if (ST == 3 && t + 1 < t1) stage_barrier<LA + LB>();
+        else stage_barrier<0>();
+        if (next < t1) issue();
         const unsigned char* As = lds + buf * kStage;
         const unsigned char* Bs = As + kA;
 #pragma unroll
@@ -278,6 +337,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
             GEOGCN_TERM(0, 0)
 #undef GEOGCN_TERM
         }
+        buf = buf + 1 == ST ? 0 : buf + 1;
     }
 
     // ---- epilogue ----
@@ -427,13 +487,13 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
 constexpr int kGradRows = 128;          // rows of a block: its partial sums are 32 sequential adds per wave, then a tree
 template <int P>
 __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn U, int64_t M, int N, int act, uint16_t* __restrict__ oG,
-                                                        uint16_t* __restrict__ oU, int64_t ldo, int64_t plane, float* __restrict__ part, int64_t part_ld) {
+                                                        uint16_t* __restrict__ oU, int cols, int64_t ldo, int64_t plane, float* __restrict__ part, int64_t part_ld) {
     __shared__ float red[4][64][8];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int c = (blockIdx.x * 64 + lane) * 4;
     const int64_t r0 = (int64_t)blockIdx.y * kGradRows, r1 = min(M, r0 + kGradRows);
     float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < ldo) {
+    if (c < cols) {                     // (the pad columns of the result are written as zeros)
         for (int64_t r = r0 + w; r < r1; r += 4) {
             float4 dg = make_float4(0.f, 0.f, 0.f, 0.f), du = dg;
             if (c < N) {
@@ -502,11 +562,11 @@ int make_planes(Arena& ar, const MatIn& m, int64_t n, int64_t F, int P, bool who
         *out = Planes{static_cast<const uint16_t*>(m.p), m.ld, 0};
         return 0;
     }
-    const int64_t ld = up(F, 64), plane = n * ld;
-    uint16_t* o = static_cast<uint16_t*>(ar.take(plane * 2 * P));
+    const int64_t plane = up(F, 64), ld = P * plane;
+    uint16_t* o = static_cast<uint16_t*>(ar.take(n * ld * 2));
     *out = Planes{o, ld, plane};
-    if (!ar.base || plane == 0) return 0;
-    const int qpr = (int)(ld / 4);
+    if (!ar.base || n * ld == 0) return 0;
+    const int qpr = (int)(plane / 4);
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(n * qpr, 256), (int64_t)kNumCU * 32);
     if (P == 3) hipLaunchKernelGGL(terms_kernel<3>, dim3(grid), dim3(256), 0, st, m, n, (int)F, qpr, o, ld, plane);
     else hipLaunchKernelGGL(terms_kernel<1>, dim3(grid), dim3(256), 0, st, m, n, (int)F, qpr, o, ld, plane);
@@ -514,11 +574,12 @@ int make_planes(Arena& ar, const MatIn& m, int64_t n, int64_t F, int P, bool who
     return 0;
 }
 
-template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, bool GATED>
+template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, int ST, bool GATED>
 int launch_tile(const TileArgs& a, hipStream_t st) {
-    constexpr int bytes = 2 * BK * 2 * (PA * BM + PB * BN);
+    constexpr int bytes = ST * BK * 2 * (PA * BM + PB * BN);
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
     static LdsAttrOnce attr;
-    auto* k = &tile_kernel<PA, PB, ASTR, BSTR, NSEG, BM, BN, BK, WM, WN, GATED>;
+    auto* k = &tile_kernel<PA, PB, ASTR, BSTR, NSEG, BM, BN, BK, WM, WN, ST, GATED>;
     if (const int rc = attr.ensure(reinterpret_cast<const void*>(k), bytes)) return rc;
     hipLaunchKernelGGL(k, dim3((unsigned)(a.n_mt * a.n_nt * a.nsplit)), dim3(WM * WN * 64), bytes, st, a);
     GEOGCN_LAUNCH_CHECK("tile_kernel");
@@ -566,8 +627,8 @@ int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
     if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
     if (!ar.base) return 0;
     t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_GATED;
-    const int rc = P == 3 ? launch_tile<3, 3, false, true, 2, BM, 2 * BNS, 32, 2, 4, true>(t, st)
-                          : launch_tile<1, 1, false, true, 2, BM, 2 * BNS, 64, 2, 4, true>(t, st);
+    const int rc = P == 3 ? launch_tile<3, 3, false, true, 2, BM, 2 * BNS, 32, 2, 4, 2, true>(t, st)
+                          : launch_tile<1, 1, false, true, 2, BM, 2 * BNS, 64, 2, 4, 3, true>(t, st);
     if (rc || c.nsplit == 1) return rc;
     return finish(t, 2, EPI_GATED, st);
 }
@@ -582,8 +643,8 @@ int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
     if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
     if (!ar.base) return 0;
     t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_STORE;
-    const int rc = P == 3 ? launch_tile<3, 3, false, false, 1, BM, BN, 32, 2, 2, false>(t, st)
-                          : launch_tile<1, 1, false, false, 1, BM, BN, 64, 2, 2, false>(t, st);
+    const int rc = P == 3 ? launch_tile<3, 3, false, false, 1, BM, BN, 32, 2, 2, 2, false>(t, st)
+                          : launch_tile<1, 1, false, false, 1, BM, BN, 64, 2, 2, 2, false>(t, st);
     if (rc || c.nsplit == 1) return rc;
     return finish(t, 1, EPI_STORE, st);
 }
@@ -600,12 +661,12 @@ int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_
     t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_STORE;
     int rc;
     if (nseg == 2) {
-        if (PA == 3) rc = launch_tile<3, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, false>(t, st);
-        else if (PB == 3) rc = launch_tile<1, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, false>(t, st);
-        else rc = launch_tile<1, 1, true, true, 2, BM, 2 * BNS, 64, 2, 4, false>(t, st);
+        if (PA == 3) rc = launch_tile<3, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, 2, false>(t, st);
+        else if (PB == 3) rc = launch_tile<1, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, 2, false>(t, st);
+        else rc = launch_tile<1, 1, true, true, 2, BM, 2 * BNS, 64, 2, 4, 3, false>(t, st);
     } else {
-        if (PB == 3) rc = launch_tile<1, 3, true, true, 1, BM, BNS, 32, 2, 4, false>(t, st);
-        else rc = launch_tile<1, 1, true, true, 1, BM, BNS, 64, 2, 4, false>(t, st);
+        if (PB == 3) rc = launch_tile<1, 3, true, true, 1, BM, BNS, 32, 2, 4, 2, false>(t, st);
+        else rc = launch_tile<1, 1, true, true, 1, BM, BNS, 64, 2, 4, 3, false>(t, st);
     }
     if (rc || c.nsplit == 1) return rc;
     return finish(t, nseg, EPI_STORE, st);
@@ -706,7 +767,7 @@ struct BwdArgs {
 };
 // P = 0: dG, dU as fp32 matrices of pitch ldo
 int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t st, uint16_t** dG_out, uint16_t** dU_out) {
-    const int64_t plane = b.M * ldo, bytes = P ? plane * 2 * P : plane * 4;
+    const int64_t ldt = P ? P * ldo : ldo, plane = ldo, bytes = b.M * ldt * (P ? 2 : 4);
     uint16_t* dG = *dG_out = static_cast<uint16_t*>(ar.take(bytes));
     uint16_t* dU = *dU_out = static_cast<uint16_t*>(ar.take(bytes));
     const int64_t nparts = cdiv(b.M, kGradRows), part_ld = up(b.N, 4);
@@ -714,7 +775,7 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
     if (ar.base) {
         const dim3 grid((unsigned)cdiv(ldo, 256), (unsigned)nparts);
         auto* k = P == 3 ? &gate_grad_kernel<3> : P == 1 ? &gate_grad_kernel<1> : &gate_grad_kernel<0>;
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, ldo, plane, part, part_ld);
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, part, part_ld);
         GEOGCN_LAUNCH_CHECK("gate_grad_kernel");
         if (part)
             for (int q = 0; q < 2; ++q)
@@ -758,9 +819,9 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
 int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
     if (b.precision == GEOGCN_GEMM_F32 && b.type == GEOGCN_T_F32) return backward_exact(ar, b, GEOGCN_GEMM_F32, st);
     const int P = terms_of(b.type, b.precision), PX = b.X.type == GEOGCN_T_F32 ? P : 1;
-    const int64_t ldo = up(b.N, 64), plane = b.M * ldo;
+    const int64_t plane = up(b.N, 64), ldo = P * plane;
     uint16_t *dG, *dU;
-    if (const int rc = gate_gradients(ar, b, P, ldo, st, &dG, &dU)) return rc;
+    if (const int rc = gate_gradients(ar, b, P, plane, st, &dG, &dU)) return rc;
     if (b.dX) {
         Planes wg, wu;
         if (const int rc = make_planes(ar, b.Wg, b.K, b.N, P, true, st, &wg)) return rc;
