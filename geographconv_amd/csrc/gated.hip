@@ -115,55 +115,52 @@ __device__ __forceinline__ void store_quad(void* C, int64_t ld, int type, int64_
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(C) + row * ld + col) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
 }
 
-// One image: R output rows (or columns) by BK k-values of one term plane.
+// One image: R output rows (or columns) by the BK k-values of a stage (one or two matrix instructions deep), one term.
 template <bool STRIDED, int R, int BK>
 struct Image {
     static constexpr int kBytes = R * BK * 2;
     static constexpr int kPieces = R * BK / 8;                       // 16-byte pieces
     static constexpr int kCpr = STRIDED ? R / 8 : BK / 8;            // pieces per stored row
     static_assert(kPieces % 64 == 0, "whole wave loads");
-    // k-strided: four k-rows of a 16-lane read phase lie a stored row apart -- and a stored row may be a whole round of the banks
-    static __device__ __forceinline__ int rot(int k) {
-        if constexpr ((R * 2) % 256 == 0) return 2 * ((k & 3) + 4 * ((k >> 3) & 1));
-        else if constexpr ((R * 2) % 256 == 128) return 2 * (((k & 3) >> 1) + 2 * ((k >> 3) & 1));
-        else return 2 * ((k >> 3) & 1);
+    // k-strided: the 32 bytes (two pieces) that four lanes read of a k-row lie at pair T ^ turn(k) of the row; a read phase meets k-rows lg*8 + 0..3
+    // of two or four lane groups, and a stored row may be a whole round of the banks (R = 128) or less
+    static constexpr bool kPow2 = (R & (R - 1)) == 0;
+    static __device__ __forceinline__ int turn(int k) {
+        if constexpr (!kPow2) return R % 32 == 0 ? (k >> 3) & 1 : 0;
+        else if constexpr (R >= 128) return (k & 3) + 4 * ((k >> 3) & 1);
+        else return ((k & 3) >> 1) + 2 * ((k >> 3) & 1);
     }
-    static __device__ __forceinline__ int place(int c, int row) {   // where piece c of stored row `row` lies in that row
+    static __device__ __forceinline__ int place(int c, int row) {   // where piece c of stored row `row` lies in that row (its own inverse)
         if constexpr (!STRIDED) return BK == 64 ? (c ^ (row & 7)) : (c ^ ((row >> 1) & 3));
-        else {
-            constexpr bool pow2 = (kCpr & (kCpr - 1)) == 0;
-            if constexpr (pow2) return (c + rot(row)) & (kCpr - 1);
-            int p = c + rot(row);
-            return p >= kCpr ? p - kCpr : p;
-        }
-    }
-    static __device__ __forceinline__ int unplace(int p, int row) {
-        if constexpr (!STRIDED) return place(p, row);
-        else {
-            constexpr bool pow2 = (kCpr & (kCpr - 1)) == 0;
-            if constexpr (pow2) return (p - rot(row)) & (kCpr - 1);
-            const int c = p - rot(row);
-            return c < 0 ? c + kCpr : c;
-        }
+        else return c ^ (2 * turn(row));
     }
     // byte offset, from the image's first row and k, of the piece that belongs at place `piece` of the image
     static __device__ __forceinline__ uint32_t source(int piece, int64_t ld) {
-        const int row = piece / kCpr, c = unplace(piece - row * kCpr, row);
+        const int row = piece / kCpr, c = place(piece - row * kCpr, row);
         return (uint32_t)row * (uint32_t)(ld * 2) + (uint32_t)c * 16u;
     }
     // k-contiguous: the first of the 8 k-values of a lane's piece -- the same in every wave load (64 pieces are whole rows, and whole rounds of `place`)
-    static __device__ __forceinline__ int k_of_lane(int lane) { return unplace(lane % kCpr, lane / kCpr) * 8; }
-    // the fragment of 16 rows from r0: lane (li, lg) gets its row's k-values s*32 + lg*8 .. + 7
-    static __device__ __forceinline__ bf16x8 read(const unsigned char* img, int r0, int s, int li, int lg) {
+    static __device__ __forceinline__ int k_of_lane(int lane) { return place(lane % kCpr, lane / kCpr) * 8; }
+    // Fragments: 16 output rows (tile T of the image) by 32 k-values (k-step s); lane (li, lg) gets its row's k-values s*32 + lg*8 .. + 7.
+    // lane_base: the lane's byte address for T = 0, s = 0; images start on multiples of 1 KB, so the permutations are exclusive-ors on it.
+    static __device__ __forceinline__ uint32_t lane_base(int li, int lg) {
+        if constexpr (!STRIDED) return (uint32_t)(li * (BK * 2) + place(lg, li) * 16);
+        else {
+            const int k = lg * 8 + (li >> 2);
+            return (uint32_t)(k * (R * 2) + turn(k) * 32 + ((li & 3) >> 1) * 16 + (li & 1) * 8);
+        }
+    }
+    static __device__ __forceinline__ bf16x8 read(uint32_t base, int T, int s, int lg) {
         if constexpr (!STRIDED) {
-            const int row = r0 + li;
-            return *reinterpret_cast<const bf16x8*>(img + row * (BK * 2) + place(s * 4 + lg, row) * 16);
+            typedef __attribute__((address_space(3))) const bf16x8* lds8;
+            return *(lds8)(uintptr_t)((base ^ (uint32_t)(s * 64)) + (uint32_t)(T * 16 * BK * 2));
         } else {
             typedef __attribute__((address_space(3))) s16x4* lds4;
-            const int k = s * 32 + lg * 8 + (li >> 2), c = r0 / 8 + ((li & 3) >> 1);
-            const uint32_t a = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)img + (uint32_t)(k * (R * 2) + place(c, k) * 16 + (li & 1) * 8);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)a);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(a + 4 * R * 2));       // (rot(k + 4) == rot(k))
+            // (R = 80, 160: the row's length has bits of its own where T does; there turn is one bit, and T ^ turn is T +- turn)
+            const int t1 = R % 32 == 0 ? lg & 1 : 0;
+            const uint32_t a = kPow2 ? (base ^ (uint32_t)(T * 32)) : base + (uint32_t)(T * 32) - ((T & 1) ? (uint32_t)(t1 * 64) : 0u);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(a + (uint32_t)(s * 32 * R * 2)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(a + (uint32_t)((s * 32 + 4) * R * 2)));       // (turn(k + 4) == turn(k))
             return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
     }
@@ -176,9 +173,10 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t voff, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
 }
-// all but the newest `LEFT` of this wave's loads have landed, its LDS reads are done, and so they are in every wave of the block
+// all but the newest LEFT of this wave's loads to LDS have landed, its LDS reads are done, and so they are in every wave of the block
 template <int LEFT>
 __device__ __forceinline__ void stage_barrier() {
+    static_assert(LEFT < 64, "vmcnt");
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(LEFT) : "memory");
 }
 // where an operand is read: the address of its first row and k of the stage, and the bytes from there to the matrix' end (reads behind: zeros)
@@ -204,15 +202,19 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
     typedef Image<ASTR, BM, BK> IA;
     typedef Image<BSTR, BNS, BK> IB;
     constexpr int MT = BM / WM / 16;                          // 16-row tiles of a wave
-    constexpr int CW = BNS / WN, NTS = CW / 16, NT = NTS * NSEG;
-    static_assert(BM % (WM * 16) == 0 && CW % 16 == 0 && (!GATED || (NSEG == 2 && CW % 32 == 0)), "wave tiles");
+    // columns: in the gated product a wave owns CW columns of both segments, otherwise the waves of a row share the segments out among them
+    constexpr bool PAIR = GATED || NSEG == 1;
+    constexpr int WNS = PAIR ? WN : WN / 2;                   // waves side by side over a segment
+    constexpr int CW = BNS / WNS, NTS = CW / 16, NT = GATED ? NTS * 2 : NTS;
+    static_assert(BM % (WM * 16) == 0 && CW % 16 == 0 && BNS % WNS == 0 && (PAIR || WN % 2 == 0) && (!GATED || (NSEG == 2 && CW % 32 == 0)), "wave tiles");
     constexpr int kA = PA * IA::kBytes, kStage = kA + PB * NSEG * IB::kBytes;
     constexpr int LIA = IA::kPieces / 64, LIB = IB::kPieces / 64;                   // wave loads of an image
-    constexpr int LA = PA * LIA / NW, LB = PB * NSEG * LIB / NW;                    // ... of a stage, per wave
-    static_assert(PA * LIA % NW == 0 && PB * LIB % NW == 0, "every wave loads as much of each operand");
+    constexpr int TA = PA * LIA, TB = PB * LIB * NSEG;                              // ... of a stage
+    constexpr int LA = (TA + NW - 1) / NW, LB = (TB + NW - 1) / NW;                 // ... of a stage, per wave (at most)
+    static_assert(ST == 2 || (TA % NW == 0 && TB % NW == 0), "a wait that leaves loads open counts on every wave having asked for as many");
     extern __shared__ __attribute__((aligned(128))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 15, lg = lane >> 4, wm = wid / WN, wn = wid % WN;
+    const int li = lane & 15, lg = lane >> 4, wm = wid / WN, wn = PAIR ? wid % WN : wid % WN % WNS, wseg = PAIR ? 0 : wid % WN / WNS;
 
     // tile of this block: every XCD works on a run of neighbouring tiles (blocks go round the XCDs one by one), taken in groups of 8 row tiles
     // so that the operands of the tiles in flight fit that XCD's L2
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
     const int mt = first + in % rows_in, nt = in / rows_in;
     const int64_t m0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNS;
 
-    const int ns0 = (int)((a.K[0] + BK - 1) / BK), nsteps = ns0 + (a.n_kseg == 2 ? (int)((a.K[1] + BK - 1) / BK) : 0);
+    const int ns0 = (int)((a.K[0] + BK - 1) / BK), nsteps = max(1, ns0 + (a.n_kseg == 2 ? (int)((a.K[1] + BK - 1) / BK) : 0));      // (no k at all: one stage of zeros)
     const int t0 = z * a.steps_per_split, t1 = min(nsteps, t0 + a.steps_per_split);
 
     f32x4 acc[MT][NT];
@@ -237,11 +239,16 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // this wave's loads of a stage: LA pieces of A's images, then LB of B's (segment by segment), 64 x 16 bytes each
+    // this wave's loads of a stage: LA pieces of A's images, LB of B's (both segments'), 64 x 16 bytes each
     uint32_t va[LA], vb[LB];
     const int ka = IA::k_of_lane(lane), kb = IB::k_of_lane(lane);
     Cursor ca, cb[NSEG];
     int64_t k_left;
+    auto seg_of = [&](int i) __attribute__((always_inline)) {                // the segment of B that this wave's load i belongs to
+        if constexpr (NSEG == 1) return 0;
+        else if constexpr (PB * LIB % NW == 0) return i / (PB * LIB / NW);
+        else return i * NW + wid >= PB * LIB ? 1 : 0;
+    };
     auto start = [&](int ks, int step) __attribute__((always_inline)) {      // cursors at stage `step` of reduction segment ks
         const int64_t k0 = (int64_t)step * BK, K = a.K[ks];
         const int64_t lda = a.lda[ks];
@@ -262,8 +269,9 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < LB; ++i) {
-            const int l = i % (LB / NSEG) * NW + wid, p = l / LIB;
-            vb[i] = IB::source((l - p * LIB) * 64 + lane, a.ldb[NSEG == 2 ? i / (LB / NSEG) : ks]) + (uint32_t)(p * a.planeB[NSEG == 2 ? 0 : ks] * 2);
+            const int q = seg_of(i), l = i * NW + wid - q * (PB * LIB), p = l / LIB;
+            const int64_t ldb = NSEG == 2 ? (q ? a.ldb[1] : a.ldb[0]) : a.ldb[ks];
+            vb[i] = IB::source((l - p * LIB) * 64 + lane, ldb) + (uint32_t)(p * a.planeB[NSEG == 2 ? 0 : ks] * 2);
         }
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + (uint32_t)wid * 1024u;
@@ -280,13 +288,15 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
         for (int i = 0; i < LA; ++i) {
             uint32_t v = va[i];
             if (!ASTR && tail) v = ka < k_left ? v : kOob;
+            if (TA % NW != 0 && i * NW + wid >= TA) continue;
             load_to_lds(ra, v, to + (uint32_t)(i * NW * 1024));
         }
 #pragma unroll
         for (int i = 0; i < LB; ++i) {
             uint32_t v = vb[i];
             if (!BSTR && tail) v = kb < k_left ? v : kOob;
-            load_to_lds(rb[i / (LB / NSEG)], v, to + (uint32_t)(kA + i * NW * 1024));
+            if (TB % NW != 0 && i * NW + wid >= TB) continue;
+            load_to_lds(NSEG == 1 || seg_of(i) == 0 ? rb[0] : rb[NSEG - 1], v, to + (uint32_t)(kA + i * NW * 1024));
         }
         const int ks = a.n_kseg == 2 && next >= ns0 ? 1 : 0;
         ca.advance(ASTR ? (int64_t)BK * 2 * a.lda[ks] : BK * 2);
@@ -297,48 +307,98 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
         fill = fill + 1 == ST ? 0 : fill + 1;
     };
 
-    if (t0 < t1) {
-        if (a.n_kseg == 2 && t0 > ns0) start(1, t0 - ns0);
-        else start(0, t0);                                    // (t0 == ns0: issue() starts the second segment)
+    if (a.n_kseg == 2 && t0 > ns0) start(1, t0 - ns0);
+    else start(0, t0);                                        // (t0 == ns0: issue() starts the second segment)
+
+    // Two phases a stage (BK = 32: the first and the second half of the wave's columns; BK = 64: of the k-values), with the stage's barrier BETWEEN
+    // them: the second phase's fragments are read while the first one's products run, so at the barrier this stage's buffer is free -- the stage ST further on is asked for at
+    // once -- and the next stage's first fragments are read while the second phase's products run.  No product waits for an LDS read that
+    // was not issued a phase ahead.  At BK = 32 A is held once: in the second phase its fragments are refilled in the order in which they are
+    // used up.
+    // Operands swapped, so that a lane owns 4 consecutive columns of one row of C; cross products of three terms from the small ones up.
+#define GEOGCN_MFMA(A_, B_, J0, i, j, pa, pb) acc[i][J0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(B_[j][pb], A_[i][pa], acc[i][J0 + j], 0, 0, 0);
+#define GEOGCN_TERM(A_, B_, J0, JN, pa, pb) \
+    _Pragma("unroll") for (int i = 0; i < MT; ++i) _Pragma("unroll") for (int j = 0; j < JN; ++j) GEOGCN_MFMA(A_, B_, J0, i, j, pa, pb)
+#define GEOGCN_TERMS(A_, B_, J0, JN, REFILL)                                                                                               \
+    if constexpr (PA == 3) {                                                                                                           \
+        GEOGCN_TERM(A_, B_, J0, JN, 2, 0) _Pragma("unroll") for (int i = 0; i < MT; ++i) { REFILL(i, 2) }                                  \
+        GEOGCN_TERM(A_, B_, J0, JN, 1, 1) GEOGCN_TERM(A_, B_, J0, JN, 1, 0) _Pragma("unroll") for (int i = 0; i < MT; ++i) { REFILL(i, 1) }    \
+        GEOGCN_TERM(A_, B_, J0, JN, 0, 2) GEOGCN_TERM(A_, B_, J0, JN, 0, 1)                                                                    \
+        _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                               \
+            _Pragma("unroll") for (int j = 0; j < JN; ++j) GEOGCN_MFMA(A_, B_, J0, i, j, 0, 0)                                         \
+            REFILL(i, 0)                                                                                                               \
+        }                                                                                                                              \
+    } else {                                                                                                                           \
+        _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                               \
+            _Pragma("unroll") for (int pb = PB - 1; pb >= 0; --pb) _Pragma("unroll") for (int j = 0; j < JN; ++j) GEOGCN_MFMA(A_, B_, J0, i, j, 0, pb) \
+            REFILL(i, 0)                                                                                                               \
+        }                                                                                                                              \
+    }
+#define GEOGCN_NO_REFILL(i, p)
+#define GEOGCN_REFILL(i, p) fa[i][p] = IA::read(la + at + (uint32_t)((p) * IA::kBytes), wm * MT + i, 0, lg);
+    constexpr bool BYK = BK == 64;
+    static_assert(BK == 32 || (PA == 1 && PB == 1), "two k-steps a stage: one term");
+    constexpr int N0 = BYK ? NT : (NT + 1) / 2, N1 = BYK ? NT : NT - N0, J1 = BYK ? 0 : N0;       // columns of the two phases, in tiles
+    bf16x8 fa[MT][PA], fa1[BYK ? MT : 1][PA], b0[N0][PB], b1[N1][PB];
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+    const uint32_t la = lds_at + IA::lane_base(li, lg), lb = lds_at + kA + IB::lane_base(li, lg) + (uint32_t)(PAIR ? 0 : wseg * PB * IB::kBytes);
+    uint32_t at = 0;                                          // the buffer of the stage at hand
+    auto read_b = [&](auto& f, int s, int j0, int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < n; ++j)
+#pragma unroll
+            for (int p = 0; p < PB; ++p)
+                f[j][p] = IB::read(lb + at + (uint32_t)(((PAIR ? (j0 + j) / NTS : 0) * PB + p) * IB::kBytes), wn * NTS + (j0 + j) % NTS, s, lg);
+    };
+    auto second = [&]() __attribute__((always_inline)) {      // the second phase's fragments
+        if constexpr (BYK) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fa1[i][0] = IA::read(la + at, wm * MT + i, 1, lg);
+        }
+        read_b(b1, BYK ? 1 : 0, J1, N1);
+    };
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+        if (i == ST - 1) {                                    // the first stage has landed (its buffer is not the one asked for next)
+            if (t0 + ST - 1 <= t1) stage_barrier<(ST - 2) * (LA + LB)>();
+            else stage_barrier<0>();
+        }
+        if (next < t1) issue();
     }
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i)
-        if (t0 + i < t1) issue();
-    int buf = 0;
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int p = 0; p < PA; ++p) { GEOGCN_REFILL(i, p) }
+    read_b(b0, 0, 0, N0);
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
-        // stage t has landed, and nobody reads the buffer of stage t - 1 any more
-        if (ST == 3 && t + 1 < t1) stage_barrier<LA + LB>();
+    for (int t = t0; t + 1 < t1; ++t) {
+        second();
+        GEOGCN_TERMS(fa, b0, 0, N0, GEOGCN_NO_REFILL)
+        // stage t + 1 has landed: of the stages asked for so far, up to t + ST - 1, the ones behind it may be on their way
+        if (t + ST <= t1) stage_barrier<(ST - 2) * (LA + LB)>();
         else stage_barrier<0>();
         if (next < t1) issue();
-        const unsigned char* As = lds + buf * kStage;
-        const unsigned char* Bs = As + kA;
+        at = at + kStage == ST * kStage ? 0 : at + kStage;
+        // (opaque: addresses are formed where they are used instead of living in registers across the loop)
+        asm volatile("" : "+s"(at));
+        read_b(b0, 0, 0, N0);
+        if constexpr (BYK) {
 #pragma unroll
-        for (int s = 0; s < BK / 32; ++s) {
-            bf16x8 af[MT][PA], bf[NT][PB];
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int p = 0; p < PA; ++p) af[i][p] = IA::read(As + p * IA::kBytes, (wm * MT + i) * 16, s, li, lg);
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int p = 0; p < PB; ++p)
-                    bf[j][p] = IB::read(Bs + ((j / NTS) * PB + p) * IB::kBytes, wn * CW + (j % NTS) * 16, s, li, lg);
-            // cross products, smallest first; operands swapped, so that a lane owns 4 consecutive columns of one row of C
-#define GEOGCN_TERM(pa, pb)                                                       \
-    _Pragma("unroll") for (int i = 0; i < MT; ++i) _Pragma("unroll") for (int j = 0; j < NT; ++j) \
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][pb], af[i][pa], acc[i][j], 0, 0, 0);
-            if constexpr (PA == 3 && PB == 3) {
-                GEOGCN_TERM(2, 0) GEOGCN_TERM(0, 2) GEOGCN_TERM(1, 1) GEOGCN_TERM(1, 0) GEOGCN_TERM(0, 1)
-            } else if constexpr (PB == 3) {
-                GEOGCN_TERM(0, 2) GEOGCN_TERM(0, 1)
-            }
-            GEOGCN_TERM(0, 0)
-#undef GEOGCN_TERM
+            for (int i = 0; i < MT; ++i) { GEOGCN_REFILL(i, 0) }
+            GEOGCN_TERMS(fa1, b1, J1, N1, GEOGCN_NO_REFILL)
+        } else {
+            GEOGCN_TERMS(fa, b1, J1, N1, GEOGCN_REFILL)
         }
-        buf = buf + 1 == ST ? 0 : buf + 1;
     }
+    second();
+    GEOGCN_TERMS(fa, b0, 0, N0, GEOGCN_NO_REFILL)
+    if constexpr (BYK) { GEOGCN_TERMS(fa1, b1, J1, N1, GEOGCN_NO_REFILL) }
+    else { GEOGCN_TERMS(fa, b1, J1, N1, GEOGCN_NO_REFILL) }
+#undef GEOGCN_REFILL
+#undef GEOGCN_NO_REFILL
+#undef GEOGCN_TERMS
+#undef GEOGCN_TERM
+#undef GEOGCN_MFMA
 
     // ---- epilogue ----
     if constexpr (GATED) {
@@ -410,7 +470,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
         if (row >= a.M) continue;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int q = j / NTS;
+            const int q = PAIR ? j / NTS : wseg;
             const int64_t col = n0 + wn * CW + (j % NTS) * 16 + lg * 4;
             float x[4];
 #pragma unroll
@@ -484,14 +544,14 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
 }
 
 // ---- dG, dU as term planes (P = 0: as fp32 matrices), with the partial column sums of both (bias gradients) ------------------------------
-constexpr int kGradRows = 128;          // rows of a block: its partial sums are 32 sequential adds per wave, then a tree
+// A block takes `rows` rows of 256 columns; its partial sums are rows / 4 sequential adds per wave, then a tree.
 template <int P>
 __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn U, int64_t M, int N, int act, uint16_t* __restrict__ oG,
-                                                        uint16_t* __restrict__ oU, int cols, int64_t ldo, int64_t plane, float* __restrict__ part, int64_t part_ld) {
+                                                        uint16_t* __restrict__ oU, int cols, int64_t ldo, int64_t plane, int rows, float* __restrict__ part, int64_t part_ld) {
     __shared__ float red[4][64][8];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int c = (blockIdx.x * 64 + lane) * 4;
-    const int64_t r0 = (int64_t)blockIdx.y * kGradRows, r1 = min(M, r0 + kGradRows);
+    const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = min(M, r0 + rows);
     float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < cols) {                     // (the pad columns of the result are written as zeros)
         for (int64_t r = r0 + w; r < r1; r += 4) {
@@ -537,6 +597,24 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn
         for (int k = 0; k < 4; ++k) s[k] = (red[0][lane][w * 4 + k] + red[1][lane][w * 4 + k]) + (red[2][lane][w * 4 + k] + red[3][lane][w * 4 + k]);
         *reinterpret_cast<float4*>(part + ((int64_t)w * gridDim.y + blockIdx.y) * part_ld + c) = make_float4(s[0], s[1], s[2], s[3]);
     }
+}
+
+// column sums of the partials: 64 columns a block, its four waves take every fourth part each (grid.y: dbg, dbu)
+__global__ __launch_bounds__(256) void bias_sum_kernel(const float* __restrict__ part, int nparts, int64_t part_ld, int N, float* __restrict__ d0, float* __restrict__ d1) {
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    if (c < N) {
+        const float* p = part + (int64_t)blockIdx.y * nparts * part_ld + c;
+        int i = w;
+        for (; i + 12 < nparts; i += 16) {
+            s0 += p[(int64_t)i * part_ld]; s1 += p[(int64_t)(i + 4) * part_ld]; s2 += p[(int64_t)(i + 8) * part_ld]; s3 += p[(int64_t)(i + 12) * part_ld];
+        }
+        for (; i < nparts; i += 4) s0 += p[(int64_t)i * part_ld];
+    }
+    red[w][lane] = (s0 + s1) + (s2 + s3);
+    __syncthreads();
+    if (w == 0 && c < N) (blockIdx.y ? d1 : d0)[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------------------
@@ -588,17 +666,6 @@ int launch_tile(const TileArgs& a, hipStream_t st) {
 
 // how a product is cut: tiles of the output, and its reduction over `nsplit` blocks where the tiles alone leave CUs idle
 struct Cut { int n_mt, n_nt, nsplit, steps; };
-Cut cut_of(int64_t M, int64_t ncols, int64_t bm, int64_t bns, int64_t steps) {
-    Cut c;
-    c.n_mt = (int)cdiv(M, bm);
-    c.n_nt = (int)cdiv(ncols, bns);
-    const int64_t tiles = (int64_t)c.n_mt * c.n_nt;
-    int64_t want = tiles >= kNumCU ? 1 : kNumCU / tiles;
-    want = std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));             // at least four stages a block
-    c.steps = (int)cdiv(std::max<int64_t>(steps, 1), want);
-    c.nsplit = (int)std::max<int64_t>(1, cdiv(steps, c.steps));
-    return c;
-}
 
 int64_t out_cols(int type, int64_t N, int64_t ld) { return std::min<int64_t>(ld, up(N, type == GEOGCN_T_F32 ? 4 : 64)); }
 
@@ -617,59 +684,88 @@ int finish(const TileArgs& t, int nseg, int mode, hipStream_t st) {
     return 0;
 }
 
-// X.[Wg | Wu] and the gate
-int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
-    constexpr int BM = 128, BNS = 128;
-    const int64_t bk = P == 3 ? 32 : 64;
-    const Cut c = cut_of(t.M, std::max(t.ncols, t.keep == GEOGCN_KEEP_MX8 ? up(t.N, kMxBlock) : 0), BM, BNS, cdiv(t.K[0], bk));
+// one product on one tile shape: run it, and add up what was split
+template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK, int WM, int WN, int ST, bool GATED>
+int run_tiles(Arena& ar, TileArgs& t, const Cut& c, hipStream_t st) {
     t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
-    t.segw = (int64_t)c.n_nt * BNS; t.ldw = 2 * t.segw;
+    t.segw = (int64_t)c.n_nt * (BN / NSEG); t.ldw = NSEG * t.segw;
     if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
     if (!ar.base) return 0;
-    t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_GATED;
-    const int rc = P == 3 ? launch_tile<3, 3, false, true, 2, BM, 2 * BNS, 32, 2, 4, 2, true>(t, st)
-                          : launch_tile<1, 1, false, true, 2, BM, 2 * BNS, 64, 2, 4, 3, true>(t, st);
+    t.mode = c.nsplit > 1 ? EPI_SLAB : GATED ? EPI_GATED : EPI_STORE;
+    const int rc = launch_tile<PA, PB, ASTR, BSTR, NSEG, BM, BN, BK, WM, WN, ST, GATED>(t, st);
     if (rc || c.nsplit == 1) return rc;
-    return finish(t, 2, EPI_GATED, st);
+    return finish(t, NSEG, GATED ? EPI_GATED : EPI_STORE, st);
 }
 
-// dG.Wg^T + dU.Wu^T
+// Which tile shape, and how many ways the reduction is split: the pair with the least estimated time, in clocks -- the busiest CU's share of
+// the products at half of the matrix pipe's rate times the shape's measured standing (`eff`: 1 for the fastest of its list on a large product),
+// plus, for a split, its slabs written and read back at the rate of a large copy and one more launch.
+struct Shape {
+    int bm, bns, bk;
+    double eff;
+    int (*run)(Arena&, TileArgs&, const Cut&, hipStream_t);
+};
+template <int N>
+int run_best(const Shape (&shapes)[N], Arena& ar, TileArgs& t, int64_t cols, int nseg, int terms, hipStream_t st) {
+    double best = 0;
+    const Shape* pick = nullptr;
+    Cut cut{};
+    for (const Shape& s : shapes) {
+        const int64_t n_mt = cdiv(t.M, s.bm), n_nt = cdiv(cols, s.bns), tiles = n_mt * n_nt;
+        const int64_t steps = std::max<int64_t>(1, t.n_kseg * cdiv(t.K[0], s.bk));
+        for (int64_t want = 1; want == 1 || (want <= steps / 4 && tiles * want <= 2 * kNumCU); want += want < 8 ? 1 : want / 4) {
+            const int64_t per = cdiv(steps, want), nsplit = cdiv(steps, per);
+            double clk = (double)cdiv(tiles * nsplit, kNumCU) * s.bm * s.bns * nseg * (per * s.bk) * terms / (2048 * 0.5 * s.eff);
+            if (nsplit > 1) clk += 2.0 * nsplit * t.M * n_nt * s.bns * nseg * 4 / 2200 + 8000;
+            if (!pick || clk < best) {
+                best = clk;
+                pick = &s;
+                cut = Cut{(int)n_mt, (int)n_nt, (int)nsplit, (int)per};
+            }
+        }
+    }
+    return pick->run(ar, t, cut, st);
+}
+
+// X.[Wg | Wu] and the gate.  (Shapes of two blocks a CU where LDS and registers allow: one block's epilogue and barriers run under the other's
+// products.  8192 x 2048 -> 8192 in bf16: 128 x 256 531-660 us by box, the same with 64 k-values a stage and one block a CU 650-790.)
+int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
+    static const Shape fp32[] = {{128, 128, 32, 1.0, run_tiles<3, 3, false, true, 2, 128, 256, 32, 2, 4, 2, true>},
+                                 {256, 64, 32, 0.95, run_tiles<3, 3, false, true, 2, 256, 128, 32, 4, 2, 2, true>},
+                                 {64, 64, 32, 0.85, run_tiles<3, 3, false, true, 2, 64, 128, 32, 2, 2, 2, true>}};
+    static const Shape bf16[] = {{128, 128, 32, 1.0, run_tiles<1, 1, false, true, 2, 128, 256, 32, 2, 4, 3, true>},
+                                 {256, 64, 32, 0.97, run_tiles<1, 1, false, true, 2, 256, 128, 32, 4, 2, 3, true>},
+                                 {128, 64, 32, 0.88, run_tiles<1, 1, false, true, 2, 128, 128, 32, 4, 2, 3, true>}};
+    const int64_t cols = t.keep == GEOGCN_KEEP_MX8 ? std::max(t.ncols, up(t.N, kMxBlock)) : t.ncols;
+    return P == 3 ? run_best(fp32, ar, t, cols, 2, 6, st) : run_best(bf16, ar, t, cols, 2, 1, st);
+}
+
+// dG.Wg^T + dU.Wu^T: both operands run along k, so the one-term shapes take 64 k-values a stage (whole 128-byte lines of a row)
 int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
-    constexpr int BM = 128, BN = 128;
-    const int64_t bk = P == 3 ? 32 : 64;
-    const Cut c = cut_of(t.M, t.ncols, BM, BN, 2 * cdiv(t.K[0], bk));
-    t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
-    t.segw = (int64_t)c.n_nt * BN; t.ldw = t.segw;
-    if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
-    if (!ar.base) return 0;
-    t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_STORE;
-    const int rc = P == 3 ? launch_tile<3, 3, false, false, 1, BM, BN, 32, 2, 2, 2, false>(t, st)
-                          : launch_tile<1, 1, false, false, 1, BM, BN, 64, 2, 2, 2, false>(t, st);
-    if (rc || c.nsplit == 1) return rc;
-    return finish(t, 1, EPI_STORE, st);
+    static const Shape fp32[] = {{256, 160, 32, 1.0, run_tiles<3, 3, false, false, 1, 256, 160, 32, 4, 2, 2, false>},
+                                 {256, 128, 32, 0.92, run_tiles<3, 3, false, false, 1, 256, 128, 32, 4, 2, 2, false>},
+                                 {64, 128, 32, 0.68, run_tiles<3, 3, false, false, 1, 64, 128, 32, 2, 2, 2, false>}};
+    static const Shape bf16[] = {{256, 256, 64, 1.0, run_tiles<1, 1, false, false, 1, 256, 256, 64, 2, 4, 2, false>},
+                                 {256, 128, 64, 0.85, run_tiles<1, 1, false, false, 1, 256, 128, 64, 4, 2, 3, false>},
+                                 {128, 128, 64, 0.8, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 2, false>}};
+    return P == 3 ? run_best(fp32, ar, t, t.ncols, 1, 6, st) : run_best(bf16, ar, t, t.ncols, 1, 1, st);
 }
 
 // X^T.[B0 | B1] (nseg = 2) or X^T.B0
 int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_t st) {
-    constexpr int BM = 128, BNS = 128;
-    const int64_t bk = PB == 3 ? 32 : 64;
-    const Cut c = cut_of(t.M, t.ncols, BM, BNS, cdiv(t.K[0], bk));
-    t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
-    t.segw = (int64_t)c.n_nt * BNS; t.ldw = nseg * t.segw;
-    if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
-    if (!ar.base) return 0;
-    t.mode = c.nsplit > 1 ? EPI_SLAB : EPI_STORE;
-    int rc;
+    static const Shape fp32[] = {{128, 128, 32, 1.0, run_tiles<3, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
+    static const Shape mx8[] = {{160, 160, 32, 1.0, run_tiles<1, 3, true, true, 2, 160, 320, 32, 2, 4, 2, false>},
+                                {128, 128, 32, 0.85, run_tiles<1, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
+    static const Shape bf16[] = {{128, 128, 64, 1.0, run_tiles<1, 1, true, true, 2, 128, 256, 64, 2, 4, 2, false>},
+                                 {128, 64, 64, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 2, 2, false>}};
+    static const Shape mx8_one[] = {{160, 256, 32, 1.0, run_tiles<1, 3, true, true, 1, 160, 256, 32, 2, 4, 2, false>},
+                                    {128, 128, 32, 0.8, run_tiles<1, 3, true, true, 1, 128, 128, 32, 2, 4, 5, false>}};
+    static const Shape bf16_one[] = {{128, 128, 32, 1.0, run_tiles<1, 1, true, true, 1, 128, 128, 32, 2, 4, 6, false>}};
     if (nseg == 2) {
-        if (PA == 3) rc = launch_tile<3, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, 2, false>(t, st);
-        else if (PB == 3) rc = launch_tile<1, 3, true, true, 2, BM, 2 * BNS, 32, 2, 4, 2, false>(t, st);
-        else rc = launch_tile<1, 1, true, true, 2, BM, 2 * BNS, 64, 2, 4, 3, false>(t, st);
-    } else {
-        if (PB == 3) rc = launch_tile<1, 3, true, true, 1, BM, BNS, 32, 2, 4, 2, false>(t, st);
-        else rc = launch_tile<1, 1, true, true, 1, BM, BNS, 64, 2, 4, 3, false>(t, st);
+        if (PA == 3) return run_best(fp32, ar, t, t.ncols, 2, 6, st);
+        return PB == 3 ? run_best(mx8, ar, t, t.ncols, 2, 3, st) : run_best(bf16, ar, t, t.ncols, 2, 1, st);
     }
-    if (rc || c.nsplit == 1) return rc;
-    return finish(t, nseg, EPI_STORE, st);
+    return PB == 3 ? run_best(mx8_one, ar, t, t.ncols, 1, 3, st) : run_best(bf16_one, ar, t, t.ncols, 1, 1, st);
 }
 
 TileArgs tile_args() {
@@ -770,16 +866,21 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
     const int64_t ldt = P ? P * ldo : ldo, plane = ldo, bytes = b.M * ldt * (P ? 2 : 4);
     uint16_t* dG = *dG_out = static_cast<uint16_t*>(ar.take(bytes));
     uint16_t* dU = *dU_out = static_cast<uint16_t*>(ar.take(bytes));
-    const int64_t nparts = cdiv(b.M, kGradRows), part_ld = up(b.N, 4);
+    // rows of a block: enough blocks to keep every CU at eight, and 1,024 rows where they are long anyway
+    const int64_t cblocks = cdiv(ldo, 256);
+    const int rows = (int)std::max(std::min<int64_t>(1024, std::max<int64_t>(4, up(cdiv(b.M * cblocks, (int64_t)kNumCU * 8), 4))),
+                                   up(cdiv(b.M, 65535), 4));          // (grid.y)
+    const int64_t nparts = cdiv(b.M, rows), part_ld = up(b.N, 4);
     float* part = b.db[0] ? static_cast<float*>(ar.take(2 * nparts * part_ld * 4)) : nullptr;
     if (ar.base) {
-        const dim3 grid((unsigned)cdiv(ldo, 256), (unsigned)nparts);
+        const dim3 grid((unsigned)cblocks, (unsigned)nparts);
         auto* k = P == 3 ? &gate_grad_kernel<3> : P == 1 ? &gate_grad_kernel<1> : &gate_grad_kernel<0>;
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, part, part_ld);
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, rows, part, part_ld);
         GEOGCN_LAUNCH_CHECK("gate_grad_kernel");
-        if (part)
-            for (int q = 0; q < 2; ++q)
-                if (const int rc = colsum_final_launch((int)nparts, (int)b.N, part + q * nparts * part_ld, part_ld, b.db[q], st)) return rc;
+        if (part) {
+            hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)cdiv(b.N, 64), 2), dim3(256), 0, st, part, (int)nparts, part_ld, (int)b.N, b.db[0], b.db[1]);
+            GEOGCN_LAUNCH_CHECK("bias_sum_kernel");
+        }
     }
     return 0;
 }
