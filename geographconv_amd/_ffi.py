@@ -15,6 +15,7 @@ ACT_NONE, ACT_TANH, ACT_SIGMOID, ACT_SELU, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 
 GEMM_F32, GEMM_BF16X3, GEMM_BF16 = 0, 1, 2
 T_F32, T_BF16, T_MX8 = 0, 1, 2
 KEEP_NONE, KEEP_FULL, KEEP_MX8 = 0, 1, 2
+E_WORKSPACE = -5
 
 c_i32, c_i64, c_f32, c_sz, c_ptr = C.c_int32, C.c_int64, C.c_float, C.c_size_t, C.c_void_p
 c_u64 = C.c_uint64

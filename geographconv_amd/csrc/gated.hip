@@ -484,6 +484,150 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
     }
 }
 
+// ---- a few rows (a served token): the weights' bytes are all there is to move -----------------------------------------------------------------
+// A block takes 32 columns of both weights over the whole reduction; its 512 threads read 16 bytes (VEC values) of each weight a step, CL lanes
+// side by side over the columns, KS k-rows at a time, straight from the matrices (no term planes: products are fp32 fmas of the stored
+// values).  x lies in LDS as [k][row].  The partial sums meet in two rotations within 16 lanes and then in LDS, always in the same order.
+// 32 columns are one checkpoint block of a row.  Bound by the latency of the one pass over the weights: 1 x 1024 -> 4096 in bf16 (16.8 MB).
+struct FewArgs {
+    int64_t M, ldx, ldwg, ldwu, ncols;
+    int K, N, act, out_type, keep;
+    const void *X, *Wg, *Wu;
+    const float* bias[2];
+    void* H; int64_t ldh;
+    void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else if constexpr (VEC == 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+        v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+    }
+}
+__device__ __forceinline__ float add_rotated(float v, int by8) {        // v + the value `8` (`4`) lanes on within each 16
+    const int x = __float_as_int(v);
+    return v + __int_as_float(by8 ? __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true) : __builtin_amdgcn_mov_dpp(x, 0x124, 0xf, 0xf, true));
+}
+template <typename T, int VEC, int RM>
+__global__ __launch_bounds__(512) void few_rows_kernel(const FewArgs a) {
+    constexpr int CL = 32 / VEC, KS = 512 / CL, KC = 1024, IT = KC / KS;
+    constexpr int U = RM <= 2 ? 8 : 4;                       // steps whose loads are in flight together
+    static_assert(IT % U == 0 && (CL == 4 || CL == 8), "layout");
+    constexpr int LDS_F = KC * RM > 32 * 64 * RM ? KC * RM : 32 * 64 * RM;
+    __shared__ __attribute__((aligned(16))) float lds[LDS_F];
+    const int tid = threadIdx.x, cl = tid % CL, ks = tid / CL, col = blockIdx.x * 32 + cl * VEC;
+    const int64_t row0 = (int64_t)blockIdx.y * RM;
+    const bool col_ok = col < a.N;
+    const T *Wg = static_cast<const T*>(a.Wg) + col, *Wu = static_cast<const T*>(a.Wu) + col, *X = static_cast<const T*>(a.X);
+    float acc[2][RM][VEC];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int r = 0; r < RM; ++r)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) acc[q][r][v] = 0.f;
+    for (int kb = 0; kb < a.K; kb += KC) {
+        float wg[U][VEC], wu[U][VEC];
+        auto fetch = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = kb + (it + u) * KS + ks;
+                if (col_ok && k < a.K) {
+                    load_vec<T, VEC>(Wg + (int64_t)k * a.ldwg, wg[u]);
+                    load_vec<T, VEC>(Wu + (int64_t)k * a.ldwu, wu[u]);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) wg[u][v] = wu[u][v] = 0.f;
+                }
+            }
+        };
+        fetch(0);                                             // (asked for before x is staged: both latencies at once)
+        const int here = min(KC, a.K - kb);
+        for (int e = tid; e < here * RM; e += 512) {
+            const int r = e / here, k = e - r * here;
+            const int64_t row = row0 + r;
+            float x = 0.f;
+            if (row < a.M) {
+                if constexpr (sizeof(T) == 4) x = X[row * a.ldx + kb + k];
+                else x = __uint_as_float((uint32_t)X[row * a.ldx + kb + k] << 16);
+            }
+            lds[k * RM + r] = x;
+        }
+        for (int e = here * RM + tid; e < KC * RM; e += 512) lds[e] = 0.f;
+        __syncthreads();
+        for (int it = 0; it * KS < here; it += U) {
+            if (it) fetch(it);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float* x = lds + ((it + u) * KS + ks) * RM;
+#pragma unroll
+                for (int r = 0; r < RM; ++r)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        acc[0][r][v] = fmaf(x[r], wg[u][v], acc[0][r][v]);
+                        acc[1][r][v] = fmaf(x[r], wu[u][v], acc[1][r][v]);
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    // 16 lanes hold 16 / CL k-rows of the same columns; the 32 groups of 16 meet in LDS as [group][q][row][column]
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int r = 0; r < RM; ++r)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                float s = acc[q][r][v];
+                if constexpr (CL == 4) s = add_rotated(s, 0);
+                s = add_rotated(s, 1);
+                if ((tid & 15) < CL) lds[((tid >> 4) * 2 + q) * (RM * 32) + r * 32 + cl * VEC + v] = s;
+            }
+    __syncthreads();
+    for (int e = tid; e < RM * 32; e += 512) {
+        const int r = e >> 5, c = blockIdx.x * 32 + (e & 31);
+        const int64_t row = row0 + r;
+        float s[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            float p[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < 32; ++g) p[g & 3] += lds[(g * 2 + q) * (RM * 32) + e];
+            s[q] = c < a.N ? (p[0] + p[1]) + (p[2] + p[3]) + (a.bias[q] ? a.bias[q][c] : 0.f) : 0.f;
+        }
+        const float h = c < a.N ? gate_value(a.act, s[0]) * s[1] : 0.f;
+        auto put = [&](void* p, int64_t ld, float x) __attribute__((always_inline)) {
+            if (a.out_type == GEOGCN_T_F32) static_cast<float*>(p)[row * ld + c] = x;
+            else static_cast<uint16_t*>(p)[row * ld + c] = (uint16_t)(pack_bf16(x, 0.f) & 0xffffu);
+        };
+        const bool in = row < a.M;
+        if (in && c < a.ncols) {
+            put(a.H, a.ldh, h);
+            if (a.keep == GEOGCN_KEEP_FULL) { put(a.keepP[0], a.ldk[0], s[0]); put(a.keepP[1], a.ldk[1], s[1]); }
+        }
+        if (a.keep == GEOGCN_KEEP_MX8) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t m = mx8_abs_bits(s[q]);
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+                const uint32_t b = mx8_scale_byte(m);
+                if (in && blockIdx.x * 32 < a.N) {
+                    static_cast<uint8_t*>(a.keepP[q])[row * a.ldk[q] + c] = (uint8_t)mx8_encode4(s[q], 0.f, 0.f, 0.f, mx8_inv_scale(b), b != 255u);
+                    if ((e & 31) == 0) a.keepS[q][row * (a.ldk[q] / kMxBlock) + blockIdx.x] = (uint8_t)b;
+                }
+            }
+        }
+    }
+}
+
 // ---- partial products of a split reduction, added in split order, and the epilogue that they were waiting for ---------------------------
 struct FinishArgs {
     int64_t M, N, segw, ldw, ncols;
@@ -620,12 +764,13 @@ __global__ __launch_bounds__(256) void bias_sum_kernel(const float* __restrict__
 // ---- host side ----------------------------------------------------------------------------------------------------------------------------
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// bump allocator over the caller's workspace; with base == nullptr it only counts
+// bump allocator over the caller's workspace; one with base == nullptr only counts (`counting`: nothing is launched)
 struct Arena {
     unsigned char* base;
+    bool counting = base == nullptr;
     size_t used = 0;
     void* take(int64_t bytes) {
-        void* p = base ? base + used : nullptr;
+        void* p = counting ? nullptr : base + used;
         used += (size_t)up(bytes, 256);
         return p;
     }
@@ -643,7 +788,7 @@ int make_planes(Arena& ar, const MatIn& m, int64_t n, int64_t F, int P, bool who
     const int64_t plane = up(F, 64), ld = P * plane;
     uint16_t* o = static_cast<uint16_t*>(ar.take(n * ld * 2));
     *out = Planes{o, ld, plane};
-    if (!ar.base || n * ld == 0) return 0;
+    if (ar.counting || n * ld == 0) return 0;
     const int qpr = (int)(plane / 4);
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(n * qpr, 256), (int64_t)kNumCU * 32);
     if (P == 3) hipLaunchKernelGGL(terms_kernel<3>, dim3(grid), dim3(256), 0, st, m, n, (int)F, qpr, o, ld, plane);
@@ -690,7 +835,7 @@ int run_tiles(Arena& ar, TileArgs& t, const Cut& c, hipStream_t st) {
     t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
     t.segw = (int64_t)c.n_nt * (BN / NSEG); t.ldw = NSEG * t.segw;
     if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
-    if (!ar.base) return 0;
+    if (ar.counting) return 0;
     t.mode = c.nsplit > 1 ? EPI_SLAB : GATED ? EPI_GATED : EPI_STORE;
     const int rc = launch_tile<PA, PB, ASTR, BSTR, NSEG, BM, BN, BK, WM, WN, ST, GATED>(t, st);
     if (rc || c.nsplit == 1) return rc;
@@ -813,6 +958,29 @@ struct FwdArgs {
     void* H; int64_t ldh;
     void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
 };
+// The rows up to which every 8 rows take one more pass over the weights (from L2) instead of term planes and whole tiles.
+constexpr int64_t kFewRows = 16;
+template <typename T, int VEC>
+int launch_few(const FewArgs& a, hipStream_t st) {
+    const int rm = a.M == 1 ? 1 : a.M == 2 ? 2 : a.M <= 4 ? 4 : 8;
+    auto* k = rm == 1 ? &few_rows_kernel<T, VEC, 1> : rm == 2 ? &few_rows_kernel<T, VEC, 2> : rm == 4 ? &few_rows_kernel<T, VEC, 4> : &few_rows_kernel<T, VEC, 8>;
+    const int64_t cols = a.keep == GEOGCN_KEEP_MX8 ? std::max(a.ncols, up(a.N, kMxBlock)) : a.ncols;
+    hipLaunchKernelGGL(k, dim3((unsigned)cdiv(cols, 32), (unsigned)cdiv(a.M, rm)), dim3(512), 0, st, a);
+    GEOGCN_LAUNCH_CHECK("few_rows_kernel");
+    return 0;
+}
+int forward_few(const FwdArgs& f, hipStream_t st) {
+    FewArgs a;
+    a.M = f.M; a.K = (int)f.K; a.N = (int)f.N; a.act = f.act; a.out_type = f.type; a.keep = f.keep;
+    a.X = f.X.p; a.ldx = f.X.ld; a.Wg = f.Wg.p; a.ldwg = f.Wg.ld; a.Wu = f.Wu.p; a.ldwu = f.Wu.ld;
+    a.bias[0] = f.bg; a.bias[1] = f.bu; a.H = f.H; a.ldh = f.ldh; a.ncols = out_cols(f.type, f.N, f.ldh);
+    for (int q = 0; q < 2; ++q) { a.keepP[q] = f.keepP[q]; a.ldk[q] = f.ldk[q]; a.keepS[q] = f.keepS[q]; }
+    if (f.type == GEOGCN_T_F32) return launch_few<float, 4>(a, st);
+    const bool wide = f.Wg.ld % 8 == 0 && f.Wu.ld % 8 == 0 && aligned16(f.Wg.p) && aligned16(f.Wu.p);
+    return wide ? launch_few<uint16_t, 8>(a, st) : launch_few<uint16_t, 4>(a, st);
+}
+bool few_rows(const FwdArgs& f) { return f.M <= kFewRows && !(f.type == GEOGCN_T_F32 && f.precision == GEOGCN_GEMM_BF16); }
+
 int forward_exact(Arena& ar, const FwdArgs& f, hipStream_t st) {
     // [G | U] by the library's dual product into one slab, the gate by the pass that finishes split reductions
     TileArgs t = tile_args();
@@ -825,7 +993,7 @@ int forward_exact(Arena& ar, const FwdArgs& f, hipStream_t st) {
     for (int q = 0; q < 2; ++q) { t.keepP[q] = f.keepP[q]; t.ldk[q] = f.ldk[q]; t.keepS[q] = f.keepS[q]; }
     const size_t need = f.K ? geogcn_gemm_dual_workspace_bytes(0, f.M, f.N, f.N, f.K, GEOGCN_GEMM_F32) : 0;
     void* w = ar.take((int64_t)need);
-    if (!ar.base) return 0;
+    if (ar.counting) return 0;
     if (f.K == 0) {
         if (const int rc = zero_rows_async(t.W, f.M, t.ldw, t.ldw, st)) return rc;
     } else if (const int rc = geogcn_gemm_dual_f32(0, f.M, f.N, f.N, f.K, static_cast<const float*>(f.X.p), f.X.ld, static_cast<const float*>(f.Wg.p),
@@ -834,6 +1002,7 @@ int forward_exact(Arena& ar, const FwdArgs& f, hipStream_t st) {
     return finish(t, 2, EPI_GATED, st);
 }
 int forward(Arena& ar, const FwdArgs& f, hipStream_t st) {
+    if (few_rows(f)) return ar.counting ? 0 : forward_few(f, st);
     if (f.precision == GEOGCN_GEMM_F32 && f.type == GEOGCN_T_F32) return forward_exact(ar, f, st);
     const int P = terms_of(f.type, f.precision);
     Planes x, wg, wu;
@@ -872,7 +1041,7 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
                                    up(cdiv(b.M, 65535), 4));          // (grid.y)
     const int64_t nparts = cdiv(b.M, rows), part_ld = up(b.N, 4);
     float* part = b.db[0] ? static_cast<float*>(ar.take(2 * nparts * part_ld * 4)) : nullptr;
-    if (ar.base) {
+    if (!ar.counting) {
         const dim3 grid((unsigned)cblocks, (unsigned)nparts);
         auto* k = P == 3 ? &gate_grad_kernel<3> : P == 1 ? &gate_grad_kernel<1> : &gate_grad_kernel<0>;
         hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, rows, part, part_ld);
@@ -893,7 +1062,7 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
     if (b.dX) {
         const size_t need = geogcn_gemm_kcat_workspace_bytes(1, b.M, b.K, b.N, b.N, precision);
         void* w = ar.take((int64_t)need);
-        if (ar.base)
+        if (!ar.counting)
             if (const int rc = geogcn_gemm_kcat_f32(1, b.M, b.K, b.N, b.N, dG, ldo, static_cast<const float*>(b.Wg.p), b.Wg.ld, dU, ldo,
                                                     static_cast<const float*>(b.Wu.p), b.Wu.ld, static_cast<float*>(b.dX), b.lddx, 0, precision,
                                                     need ? w : nullptr, need, st)) return rc;
@@ -904,13 +1073,13 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
         if (b.X.type == GEOGCN_T_MX8) {
             ldx = up(b.K, 4);
             float* x = static_cast<float*>(ar.take(b.M * ldx * 4));
-            if (ar.base)
+            if (!ar.counting)
                 if (const int rc = geogcn_mx8_unpack(b.M, (int32_t)b.K, GEOGCN_T_F32, static_cast<const uint8_t*>(b.X.p), b.X.ld, b.X.scale, x, ldx, st)) return rc;
             X = x;
         }
         const size_t need = geogcn_gemm_dual_workspace_bytes(1, b.K, b.N, b.N, b.M, precision);
         void* w = ar.take((int64_t)need);
-        if (ar.base)
+        if (!ar.counting)
             if (const int rc = geogcn_gemm_dual_f32(1, b.K, b.N, b.N, b.M, X, ldx, dG, ldo, dU, ldo, static_cast<float*>(b.dW[0]), b.lddw[0],
                                                     static_cast<float*>(b.dW[1]), b.lddw[1], nullptr, GEOGCN_ACT_NONE, nullptr, GEOGCN_ACT_NONE, precision,
                                                     need ? w : nullptr, need, st)) return rc;
@@ -958,7 +1127,7 @@ int weight_grad_exact(Arena& ar, const WgradArgs& w, hipStream_t st) {
     float* x = static_cast<float*>(ar.take(w.M * ldx * 4));
     const size_t need = geogcn_gemm_workspace_bytes(1, 0, w.K, w.N, w.M, GEOGCN_GEMM_F32);
     void* g = ar.take((int64_t)need);
-    if (!ar.base) return 0;
+    if (ar.counting) return 0;
     if (const int rc = geogcn_mx8_unpack(w.M, (int32_t)w.K, GEOGCN_T_F32, static_cast<const uint8_t*>(w.X.p), w.X.ld, w.X.scale, x, ldx, st)) return rc;
     return geogcn_gemm_f32(1, 0, w.K, w.N, w.M, x, ldx, static_cast<const float*>(w.dZ.p), w.dZ.ld, static_cast<float*>(w.dW), w.lddw, nullptr,
                            GEOGCN_ACT_NONE, 0, GEOGCN_GEMM_F32, need ? g : nullptr, need, st);
@@ -983,9 +1152,13 @@ int zero_matrix(void* p, int type, int64_t n, int64_t cols, int64_t ld, hipStrea
     return zero_rows_async(static_cast<float*>(p), n, cols / 2, ld / 2, st);
 }
 
-int check_ws(const char* who, size_t need, const void* ws, size_t have) {
-    GEOGCN_REQUIRE(need == 0 || (ws && have >= need), GEOGCN_E_ARG, "%s: workspace of %zu bytes, %zu needed", who, have, need);
-    GEOGCN_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(ws) % 256 == 0, GEOGCN_E_ALIGN, "%s: workspace not on 256 bytes", who);
+// 0: go on; else the call's return code.  *have is set to what the call needs where that is missing.
+int check_ws(const char* who, size_t need, const void* ws, size_t* have) {
+    if (need == 0) return 0;
+    const size_t got = ws ? *have : 0;
+    if (got < need) *have = need;
+    GEOGCN_REQUIRE(got >= need, GEOGCN_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, got, need);
+    GEOGCN_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0, GEOGCN_E_ALIGN, "%s: workspace not on 256 bytes", who);
     return 0;
 }
 
@@ -1028,13 +1201,9 @@ extern "C" int geogcn_gated_fwd(int64_t M, int64_t K, int64_t N, int32_t type, c
     }
     Arena count{nullptr};
     if (!empty) forward(count, f, nullptr);
-    if (!ws) {
-        *ws_bytes = std::max<size_t>(count.used, 256);
-        return 0;
-    }
     if (empty) return 0;
-    if (const int rc = check_ws(who, count.used, ws, *ws_bytes)) return rc;
-    Arena ar{static_cast<unsigned char*>(ws)};
+    if (const int rc = check_ws(who, count.used, ws, ws_bytes)) return rc;
+    Arena ar{static_cast<unsigned char*>(ws), false};
     return forward(ar, f, static_cast<hipStream_t>(stream));
 }
 
@@ -1081,10 +1250,6 @@ extern "C" int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, c
     const bool empty = M == 0 || N == 0;
     Arena count{nullptr};
     if (!empty) backward(count, b, nullptr);
-    if (!ws) {
-        *ws_bytes = std::max<size_t>(count.used, 256);
-        return 0;
-    }
     if (empty) {                                             // no rows, or no units: sums over nothing
         if (b.dX && M > 0)
             if (const int rc = zero_matrix(dX, type, M, out_cols(type, K, lddx), lddx, st)) return rc;
@@ -1096,8 +1261,8 @@ extern "C" int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, c
         }
         return 0;
     }
-    if (const int rc = check_ws(who, count.used, ws, *ws_bytes)) return rc;
-    Arena ar{static_cast<unsigned char*>(ws)};
+    if (const int rc = check_ws(who, count.used, ws, ws_bytes)) return rc;
+    Arena ar{static_cast<unsigned char*>(ws), false};
     return backward(ar, b, st);
 }
 
@@ -1119,14 +1284,10 @@ extern "C" int geogcn_mx8_weight_grad(int64_t M, int64_t K, int64_t N, int32_t t
     WgradArgs w{M, K, N, type, precision, MatIn{GEOGCN_T_MX8, X, ldx, Xs}, MatIn{type, dZ, lddz, nullptr}, dW, lddw};
     Arena count{nullptr};
     if (!none && M > 0) weight_grad(count, w, nullptr);
-    if (!ws) {
-        *ws_bytes = std::max<size_t>(count.used, 256);
-        return 0;
-    }
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (none) return 0;
     if (M == 0) return zero_matrix(dW, type, K, out_cols(type, N, lddw), lddw, st);
-    if (const int rc = check_ws(who, count.used, ws, *ws_bytes)) return rc;
-    Arena ar{static_cast<unsigned char*>(ws)};
+    if (const int rc = check_ws(who, count.used, ws, ws_bytes)) return rc;
+    Arena ar{static_cast<unsigned char*>(ws), false};
     return weight_grad(ar, w, st);
 }

@@ -1230,20 +1230,32 @@ def _mat_type(m):
 
 def _mat_args(m):
     """(pointer, pitch) of a dense matrix, (codes, pitch, scales) where a checkpoint may stand too"""
-    return (_p(m.codes), m.ld, _p(m.scales)) if isinstance(m, MX8Mat) else (_p(m.t), m.ld, C.c_void_p(0))
+    return (m.codes.data_ptr(), m.ld, m.scales.data_ptr()) if isinstance(m, MX8Mat) else (m.t.data_ptr(), m.ld, None)
 
 
-def _new_like_block(bf16, n, F, device):
-    return HMat(n, F, device) if bf16 else DMat.empty(n, F, device)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _new_like_block(bf16, n, F, device, ld=None):
+    """Uninitialised: the kernels here write the pad columns themselves."""
+    if bf16:
+        return HMat(n, F, device, ld=ld)
+    return DMat(n, F, t=torch.empty((n, ld or pad4(F)), dtype=torch.float32, device=device))
+
+
+def _tensor(m):
+    return m if m is None or isinstance(m, torch.Tensor) else m.codes if isinstance(m, MX8Mat) else m.t
 
 
 def _same_device(*ms):
-    dev = ms[0].device
-    if any(m is not None and m.device != dev for m in ms):
-        raise ValueError("operands live on different devices: %s" % sorted({str(m.device) for m in ms if m is not None}))
-    if dev.type != 'cuda':
-        raise _ffi.GeoGcnError("operands live on %s: there is no CPU path" % dev)
-    return dev
+    """-> the index of the one GPU that all operands (None: absent) live on"""
+    at = [t.get_device() for t in map(_tensor, ms) if t is not None]
+    if min(at) != max(at):
+        raise ValueError("operands live on different devices: %s" % sorted({str(_tensor(m).device) for m in ms if m is not None}))
+    if at[0] < 0:
+        raise _ffi.GeoGcnError("operands live in host memory: there is no CPU path")
+    return at[0]
 
 
 def _check_out(m, n, F, kind, what):
@@ -1258,14 +1270,29 @@ def _check_vec(v, N, what):
     return v
 
 
-def _run_with_ws(fn, name, args, dev):
-    """Ask the entry point for its scratch, allocate it for this call alone (stream-ordered; a captured call's lives in the graph's
-    pool, so two graphs never share one) and launch on the current stream of the operands' device."""
-    with torch.cuda.device(dev):
-        need = C.c_size_t(0)
-        check(fn(*args, C.c_void_p(0), C.byref(need), C.c_void_p(0)), name)
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        check(fn(*args, _p(ws), C.byref(need), _stream()), name)
+def _call(fn, name, *args):
+    """One C entry point on the current stream of the current device."""
+    check(fn(*args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())), name)
+
+
+def _call_with_ws(fn, name, *args):
+    """... of one that says what scratch it needs (GEOGCN_E_WORKSPACE): allocated for this call alone -- stream-ordered, and a captured call's
+    lives in the graph's pool, so two graphs never share one."""
+    need, st = C.c_size_t(0), torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    rc = fn(*args, None, need, st)
+    if rc == _ffi.E_WORKSPACE:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=torch.cuda.current_device())
+        rc = fn(*args, ws.data_ptr(), need, st)
+    check(rc, name)
+
+
+def _on_device(index, call, fn, name, *args):
+    """`call` (_call / _call_with_ws) with the operands' device current."""
+    if torch.cuda.current_device() == index:
+        call(fn, name, *args)
+    else:
+        with torch.cuda.device(index):
+            call(fn, name, *args)
 
 
 @_timed('mx8_pack')
@@ -1280,9 +1307,8 @@ def mx8_pack(X, out: MX8Mat = None):
         out = MX8Mat.empty(X.n, X.F, X.device, bf16)
     elif (out.n, out.F, out.bf16) != (X.n, X.F, bf16):
         raise ValueError("mx8_pack: the output does not have the input's shape and type")
-    dev = _same_device(X, out)
-    with torch.cuda.device(dev):
-        check(_ffi.lib().geogcn_mx8_pack(X.n, X.F, t, _p(X.t), X.ld, _p(out.codes), out.ld, _p(out.scales), _stream()), 'mx8_pack')
+    _on_device(_same_device(X, out), _call, _ffi.lib().geogcn_mx8_pack, 'mx8_pack', X.n, X.F, t, X.t.data_ptr(), X.ld, out.codes.data_ptr(), out.ld,
+               out.scales.data_ptr())
     return out
 
 
@@ -1293,9 +1319,8 @@ def mx8_unpack(Q: MX8Mat, out=None):
         raise ValueError("mx8_unpack: not an 8-bit checkpoint")
     kind = HMat if Q.bf16 else DMat
     out = _new_like_block(Q.bf16, Q.n, Q.F, Q.device) if out is None else _check_out(out, Q.n, Q.F, kind, 'mx8_unpack: the output')
-    dev = _same_device(Q, out)
-    with torch.cuda.device(dev):
-        check(_ffi.lib().geogcn_mx8_unpack(Q.n, Q.F, _mat_type(out), _p(Q.codes), Q.ld, _p(Q.scales), _p(out.t), out.ld, _stream()), 'mx8_unpack')
+    _on_device(_same_device(Q, out), _call, _ffi.lib().geogcn_mx8_unpack, 'mx8_unpack', Q.n, Q.F, _mat_type(out), Q.codes.data_ptr(), Q.ld,
+               Q.scales.data_ptr(), out.t.data_ptr(), out.ld)
     return out
 
 
@@ -1311,12 +1336,12 @@ def mx8_weight_grad(X: MX8Mat, dZ, out=None, precision=None):
                          % (X.n, 'bf16' if X.bf16 else 'fp32', dZ.n, 'bf16' if bf16 else 'fp32'))
     prec = _block_precision(precision, bf16)
     out = _new_like_block(bf16, X.F, dZ.F, X.device) if out is None else _check_out(out, X.F, dZ.F, HMat if bf16 else DMat, 'mx8_weight_grad: the output')
-    dev = _same_device(X, dZ, out)
-    _run_with_ws(_ffi.lib().geogcn_mx8_weight_grad, 'mx8_weight_grad',
-                 (X.n, X.F, dZ.F, _mat_type(dZ), *_mat_args(X), _p(dZ.t), dZ.ld, _p(out.t), out.ld, prec), dev)
+    _on_device(_same_device(X, dZ, out), _call_with_ws, _ffi.lib().geogcn_mx8_weight_grad, 'mx8_weight_grad', X.n, X.F, dZ.F, _mat_type(dZ),
+               *_mat_args(X), dZ.t.data_ptr(), dZ.ld, out.t.data_ptr(), out.ld, prec)
     return out
 
 
+_KEEP = {None: _ffi.KEEP_NONE, 'full': _ffi.KEEP_FULL, 'mx8': _ffi.KEEP_MX8}
 GATED_ACTS = (ACT_NONE, ACT_TANH, ACT_SIGMOID, ACT_RELU, ACT_SILU, ACT_GELU)
 
 
@@ -1359,18 +1384,16 @@ def gated_dense(X, Wg, Wu, bg: torch.Tensor = None, bu: torch.Tensor = None, act
     prec = _block_precision(precision, bf16)
     kind = HMat if bf16 else DMat
     H = _new_like_block(bf16, M, N, X.device) if out is None else _check_out(out, M, N, kind, 'gated_dense: the output')
-    dev = _same_device(X, Wg, Wu, bg, bu, H)
-    lib = _ffi.lib()
+    index = _same_device(X, Wg, Wu, bg, bu, H)
     G = U = None
     if keep == 'full':
-        G, U = (HMat(M, N, dev, ld=H.ld) if bf16 else DMat.empty(M, N, dev, ld=H.ld) for _ in range(2))
+        G, U = (_new_like_block(bf16, M, N, X.device, H.ld) for _ in range(2))
     elif keep == 'mx8':
-        G, U = MX8Mat.empty(M, N, dev, bf16), MX8Mat.empty(M, N, dev, bf16)
-    none = (C.c_void_p(0), 0, C.c_void_p(0))
-    _run_with_ws(lib.geogcn_gated_fwd, 'gated_fwd',
-                 (M, K, N, _mat_type(X), _p(X.t), X.ld, _p(Wg.t), Wg.ld, _p(Wu.t), Wu.ld, _p(bg), _p(bu), int(act), _p(H.t), H.ld,
-                  {None: _ffi.KEEP_NONE, 'full': _ffi.KEEP_FULL, 'mx8': _ffi.KEEP_MX8}[keep], *(_mat_args(G) if keep else none),
-                  *(_mat_args(U) if keep else none), prec), dev)
+        G, U = (MX8Mat.empty(M, N, X.device, bf16) for _ in range(2))
+    none = (None, 0, None)
+    _on_device(index, _call_with_ws, _ffi.lib().geogcn_gated_fwd, 'gated_fwd', M, K, N, _mat_type(X), X.t.data_ptr(), X.ld, Wg.t.data_ptr(), Wg.ld,
+               Wu.t.data_ptr(), Wu.ld, _ptr(bg), _ptr(bu), int(act), H.t.data_ptr(), H.ld, _KEEP[keep], *(_mat_args(G) if keep else none),
+               *(_mat_args(U) if keep else none), prec)
     return H if keep is None else (H, GatedTape(G, U))
 
 
@@ -1392,10 +1415,10 @@ def gated_dense_bwd(dH, X, Wg, Wu, kept: GatedTape, act=ACT_SIGMOID, dX=None, dW
         if m is not None:
             _check_out(m, n, F, kind, 'gated_dense_bwd: ' + what)
     prec = _block_precision(precision, bf16)
-    dev = _same_device(dH, X, Wg, Wu, kept.G, kept.U, dX, dWg, dWu, dbg, dbu)
+    index, dev = _same_device(dH, X, Wg, Wu, kept.G, kept.U, dX, dWg, dWu, dbg, dbu), dH.device
     bias = bias or dbg is not None
     if bias and dbg is None:
-        dbg, dbu = (torch.zeros(pad4(N), dtype=torch.float32, device=dev) for _ in range(2))
+        dbg, dbu = ((torch.zeros if N % 4 else torch.empty)(pad4(N), dtype=torch.float32, device=dev) for _ in range(2))
     for v, what in ((dbg, 'dbg'), (dbu, 'dbu')):
         _check_vec(v, pad4(N) if bias else 0, 'gated_dense_bwd: ' + what)
     if need_input_grad:
@@ -1404,8 +1427,8 @@ def gated_dense_bwd(dH, X, Wg, Wu, kept: GatedTape, act=ACT_SIGMOID, dX=None, dW
         dX = None
     if dWg is None:
         dWg, dWu = (_new_like_block(bf16, K, N, dev) for _ in range(2))
-    _run_with_ws(_ffi.lib().geogcn_gated_bwd, 'gated_bwd',
-                 (M, K, N, _mat_type(dH), _p(dH.t), dH.ld, _mat_type(X), *_mat_args(X), _p(Wg.t), Wg.ld, _p(Wu.t), Wu.ld, tk,
-                  *_mat_args(kept.G), *_mat_args(kept.U), int(act), _p(dX.t if dX is not None else None), dX.ld if dX is not None else 0,
-                  _p(dWg.t), dWg.ld, _p(dWu.t), dWu.ld, _p(dbg), _p(dbu), prec), dev)
+    _on_device(index, _call_with_ws, _ffi.lib().geogcn_gated_bwd, 'gated_bwd', M, K, N, _mat_type(dH), dH.t.data_ptr(), dH.ld, _mat_type(X),
+               *_mat_args(X), Wg.t.data_ptr(), Wg.ld, Wu.t.data_ptr(), Wu.ld, tk, *_mat_args(kept.G), *_mat_args(kept.U), int(act),
+               _ptr(dX.t if dX is not None else None), dX.ld if dX is not None else 0, dWg.t.data_ptr(), dWg.ld, dWu.t.data_ptr(), dWu.ld,
+               _ptr(dbg), _ptr(dbu), prec)
     return dX, dWg, dWu, dbg, dbu

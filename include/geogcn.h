@@ -44,6 +44,7 @@ extern "C" {
 #define GEOGCN_E_SIZE   (-2)   /* negative / inconsistent size        */
 #define GEOGCN_E_ALIGN  (-3)   /* pitch or base alignment unsupported */
 #define GEOGCN_E_ARG    (-4)   /* bad enum / flag / workspace too small */
+#define GEOGCN_E_WORKSPACE (-5) /* geogcn_gated_* / geogcn_mx8_weight_grad: *ws_bytes now says what the call needs; nothing was launched */
 
 /* epilogue selectors (lasagne.nonlinearities used on the path: gcnmodel.py:286,347,374) */
 #define GEOGCN_ACT_NONE    0   /* linear (softmax layers keep logits; softmax is its own entry) */
@@ -511,8 +512,9 @@ int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, 
  * gives NaN.)  Products of bf16 matrices are one kind, whatever `precision` says.
  * keep: what of G = X.Wg + bg and U = X.Wu + bu is stored for the backward -- nothing, in the block's type (pitch >= H's), or as 8-bit
  * checkpoints (codes G / U with pitch ldg / ldu and scales Gs / Us as geogcn_mx8_pack writes them).
- * ws: scratch.  Call with ws = NULL to have *ws_bytes set to what the call needs (no launch); then with ws (256-byte aligned) and its size.
- * How operands are read depends on their addresses: ask with the very arguments of the call.  Nothing in ws outlives the call.            */
+ * ws: scratch of *ws_bytes bytes, 256-byte aligned (may be NULL).  A call that needs more launches nothing, sets *ws_bytes to what it needs and
+ * returns GEOGCN_E_WORKSPACE; calls of a few rows need none.  How operands are read depends on their addresses: ask with the very
+ * arguments of the call.  Nothing in ws outlives the call.                                                                               */
 #define GEOGCN_KEEP_NONE 0
 #define GEOGCN_KEEP_FULL 1
 #define GEOGCN_KEEP_MX8  2

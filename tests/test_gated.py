@@ -100,8 +100,9 @@ def test_host_memory_is_refused(call):
 
 
 def _fwd(lib, **kw):
-    """geogcn_gated_fwd with plausible (never dereferenced) addresses, some of them replaced -> return code; ws = NULL: no launch."""
-    a = dict(M=8, K=16, N=32, type=0, X=4096, ldx=16, Wg=8192, ldwg=32, Wu=12288, ldwu=32, bg=None, bu=None, act=5, H=16384, ldh=32, keep=0, G=None,
+    """geogcn_gated_fwd with plausible (never dereferenced) addresses, some of them replaced -> return code, scratch asked for; without scratch a
+    call of this many rows launches nothing."""
+    a = dict(M=80, K=16, N=32, type=0, X=4096, ldx=16, Wg=8192, ldwg=32, Wu=12288, ldwu=32, bg=None, bu=None, act=5, H=16384, ldh=32, keep=0, G=None,
              ldg=0, Gs=None, U=None, ldu=0, Us=None, precision=1)
     a.update(kw)
     need = C.c_size_t(0)
@@ -110,7 +111,7 @@ def _fwd(lib, **kw):
 
 
 def test_c_entry_refusals(lib):
-    assert _fwd(lib)[0] == 0 and _fwd(lib)[1] > 0
+    assert _fwd(lib)[0] == _ffi.E_WORKSPACE and _fwd(lib)[1] > 0
     for kw, rc in ((dict(M=-1), -2), (dict(N=1 << 21), -2), (dict(type=2), -4), (dict(act=3), -4), (dict(act=7), -4), (dict(keep=3), -4),
                    (dict(precision=3), -4), (dict(X=None), -1), (dict(Wu=None), -1), (dict(H=None), -1), (dict(X=4100), -3), (dict(ldx=18), -3),
                    (dict(ldx=12), -3), (dict(ldh=28), -3), (dict(H=16392), -3), (dict(keep=1), -1), (dict(keep=2, G=64, ldg=32, U=64, ldu=32), -1),
@@ -118,11 +119,11 @@ def test_c_entry_refusals(lib):
         got = _fwd(lib, **kw)[0]
         assert got == rc, (kw, got)
         assert lib.geogcn_last_error()
-    assert lib.geogcn_gated_fwd(8, 16, 32, 0, 4096, 16, 8192, 32, 12288, 32, None, None, 5, 16384, 32, 0, None, 0, None, None, 0, None, 1, None, None,
+    assert lib.geogcn_gated_fwd(80, 16, 32, 0, 4096, 16, 8192, 32, 12288, 32, None, None, 5, 16384, 32, 0, None, 0, None, None, 0, None, 1, None, None,
                                 None) == -1
     need = C.c_size_t(0)                                     # a workspace that is too small or badly placed is turned down before any launch
-    args = (8, 16, 32, 0, 4096, 16, 8192, 32, 12288, 32, None, None, 5, 16384, 32, 0, None, 0, None, None, 0, None, 1)
-    assert lib.geogcn_gated_fwd(*args, 256, C.byref(need), None) == -4
+    args = (80, 16, 32, 0, 4096, 16, 8192, 32, 12288, 32, None, None, 5, 16384, 32, 0, None, 0, None, None, 0, None, 1)
+    assert lib.geogcn_gated_fwd(*args, 256, C.byref(need), None) == _ffi.E_WORKSPACE and need.value == _fwd(lib)[1]
     need = C.c_size_t(1 << 30)
     assert lib.geogcn_gated_fwd(*args, 264, C.byref(need), None) == -3
 
@@ -136,8 +137,9 @@ def test_bwd_and_checkpoint_entry_refusals(lib):
                  precision=1)
         a.update(kw)
         return lib.geogcn_gated_bwd(*a.values(), None, C.byref(need), None)
-    assert bwd() == 0 and bwd(dX=None) == 0 and bwd(dWg=None, dWu=None) == 0 and bwd(dbg=4096, dbu=4096) == 0
-    assert bwd(x_type=2, ldx=32, Xs=4096) == 0 and bwd(kept_type=2, Gs=4096, Us=4096) == 0
+    for kw in (dict(), dict(dX=None), dict(dWg=None, dWu=None), dict(dbg=4096, dbu=4096), dict(x_type=2, ldx=32, Xs=4096), dict(kept_type=2, Gs=4096, Us=4096)):
+        need.value = 0
+        assert bwd(**kw) == _ffi.E_WORKSPACE and need.value > 0, kw
     for kw, rc in ((dict(dWg=None), -1), (dict(dbu=4096), -1), (dict(x_type=1), -4), (dict(kept_type=1), -4), (dict(x_type=2, Xs=4096), -3),
                    (dict(kept_type=2, Gs=4096), -1), (dict(dbg=4100, dbu=4096), -3), (dict(lddx=12), -3), (dict(dH=None), -1), (dict(act=-1), -4),
                    (dict(K=-2), -2)):
