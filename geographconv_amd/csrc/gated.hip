@@ -24,12 +24,39 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kOob = 0x80000000u;
 
 // ---- the activation of the gate and its derivative -------------------------------------------------------------------------------------
+// Every epilogue element pays for these, so they are written with the hardware's exponential and reciprocal (1 ulp each); what is held is the
+// absolute error, about 1e-7 of the larger of 1 and |x| -- that of the pre-activation itself.
+__device__ __forceinline__ float exp_neg(float y) { return __builtin_amdgcn_exp2f(-1.44269504f * y); }       // e^-y, y >= 0 (its relative error grows as 1e-7 y: harmless, the value shrinks faster)
+
+// tanh: odd polynomial where 1 - e^-2|x| would cancel (|x| < 0.3; the Taylor series to x^9, next term 6e-8 x at most), else (1 - e) / (1 + e)
+__device__ __forceinline__ float tanh_fast(float x) {
+    const float a = fabsf(x), e = exp_neg(2.f * a), s = x * x;
+    const float t = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
+    const float p = fmaf(s, fmaf(s, fmaf(s, fmaf(s, 0.021869489f, -0.053968254f), 0.13333333f), -0.33333333f), 1.f) * x;
+    return a < 0.3f ? p : copysignf(t, x);
+}
+// the normal distribution at x: e = exp(-x^2 / 2), cdf = Phi(x) = e * R(t) / 2 for x < 0 (1 - that for x > 0), t = 1 / (1 + 0.3 |x|), where R is a
+// polynomial fitted here to exp(z^2) erfc(z), z = |x| / sqrt 2, over t in (0, 1] (ten terms t .. t^10, largest error 5e-9)
+__device__ __forceinline__ void normal_fast(float x, float& cdf, float& e) {
+    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
+    e = exp_neg(0.5f * x * x);
+    constexpr float k[10] = {0.239366293f, 0.239314735f, 0.218773827f, 0.165909439f, 0.162710696f, -0.098400034f, 0.305306107f, -0.394102961f, 0.197030291f, -0.035908401f};
+    float r = k[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) r = fmaf(r, t, k[i]);
+    const float q = 0.5f * e * r * t;
+    cdf = x < 0.f ? q : 1.f - q;
+}
 __device__ __forceinline__ float gate_value(int act, float x) {
     switch (act) {
         case GEOGCN_ACT_SILU: return x * apply_act<GEOGCN_ACT_SIGMOID>(x);
-        case GEOGCN_ACT_GELU: return 0.5f * x * erfcf(-0.70710678118654752f * x);
+        case GEOGCN_ACT_GELU: {
+            float c, e;
+            normal_fast(x, c, e);
+            return x * c;
+        }
         case GEOGCN_ACT_SIGMOID: return apply_act<GEOGCN_ACT_SIGMOID>(x);
-        case GEOGCN_ACT_TANH: return tanhf(x);
+        case GEOGCN_ACT_TANH: return tanh_fast(x);
         case GEOGCN_ACT_RELU: return x > 0.f ? x : (x == x ? 0.f : x);
         default: return x;
     }
@@ -43,9 +70,10 @@ __device__ __forceinline__ void gate_value_grad(int act, float x, float& v, floa
             return;
         }
         case GEOGCN_ACT_GELU: {
-            const float cdf = 0.5f * erfcf(-0.70710678118654752f * x);
-            v = x * cdf;
-            d = fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), cdf);
+            float c, e;
+            normal_fast(x, c, e);
+            v = x * c;
+            d = fmaf(x * 0.39894228f, e, c);
             return;
         }
         case GEOGCN_ACT_SIGMOID: {
@@ -54,7 +82,7 @@ __device__ __forceinline__ void gate_value_grad(int act, float x, float& v, floa
             return;
         }
         case GEOGCN_ACT_TANH: {
-            v = tanhf(x);
+            v = tanh_fast(x);
             d = fmaf(-v, v, 1.f);
             return;
         }
@@ -497,19 +525,15 @@ struct FewArgs {
     void* H; int64_t ldh;
     void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
 };
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(p);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else if constexpr (VEC == 8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
-        v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
-    }
+template <int BYTES> struct Raw { typedef uint4 type; };
+template <> struct Raw<8> { typedef uint2 type; };
+__device__ __forceinline__ void values_of(const uint4& w, float (&v)[4]) {                    // four fp32 values
+    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void values_of(const uint2& w, float (&v)[4]) { v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y); }
+__device__ __forceinline__ void values_of(const uint4& w, float (&v)[8]) {                    // eight bf16 values
+    v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+    v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
 }
 __device__ __forceinline__ float add_rotated(float v, int by8) {        // v + the value `8` (`4`) lanes on within each 16
     const int x = __float_as_int(v);
@@ -518,14 +542,16 @@ __device__ __forceinline__ float add_rotated(float v, int by8) {        // v + t
 template <typename T, int VEC, int RM>
 __global__ __launch_bounds__(512) void few_rows_kernel(const FewArgs a) {
     constexpr int CL = 32 / VEC, KS = 512 / CL, KC = 1024, IT = KC / KS;
-    constexpr int U = RM <= 2 ? 8 : 4;                       // steps whose loads are in flight together
+    constexpr int U = RM <= 2 ? 8 : RM == 4 ? 4 : VEC == 8 ? 2 : 4;      // steps whose loads are in flight together (registers)
     static_assert(IT % U == 0 && (CL == 4 || CL == 8), "layout");
     constexpr int LDS_F = KC * RM > 32 * 64 * RM ? KC * RM : 32 * 64 * RM;
     __shared__ __attribute__((aligned(16))) float lds[LDS_F];
     const int tid = threadIdx.x, cl = tid % CL, ks = tid / CL, col = blockIdx.x * 32 + cl * VEC;
     const int64_t row0 = (int64_t)blockIdx.y * RM;
-    const bool col_ok = col < a.N;
-    const T *Wg = static_cast<const T*>(a.Wg) + col, *Wu = static_cast<const T*>(a.Wu) + col, *X = static_cast<const T*>(a.X);
+    typedef typename Raw<VEC * sizeof(T)>::type raw;
+    // (columns and k-rows outside are read from inside -- the first columns, the last row -- and count as zeros)
+    const int at = col < a.N ? col : 0;
+    const T *Wg = static_cast<const T*>(a.Wg) + at, *Wu = static_cast<const T*>(a.Wu) + at, *X = static_cast<const T*>(a.X);
     float acc[2][RM][VEC];
 #pragma unroll
     for (int q = 0; q < 2; ++q)
@@ -534,45 +560,49 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const FewArgs a) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) acc[q][r][v] = 0.f;
     for (int kb = 0; kb < a.K; kb += KC) {
-        float wg[U][VEC], wu[U][VEC];
+        raw wg[U], wu[U];
         auto fetch = [&](int it) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int k = kb + (it + u) * KS + ks;
-                if (col_ok && k < a.K) {
-                    load_vec<T, VEC>(Wg + (int64_t)k * a.ldwg, wg[u]);
-                    load_vec<T, VEC>(Wu + (int64_t)k * a.ldwu, wu[u]);
-                } else {
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) wg[u][v] = wu[u][v] = 0.f;
-                }
+                const int64_t k = min(kb + (it + u) * KS + ks, a.K - 1);
+                wg[u] = *reinterpret_cast<const raw*>(Wg + k * a.ldwg);
+                wu[u] = *reinterpret_cast<const raw*>(Wu + k * a.ldwu);
             }
         };
         fetch(0);                                             // (asked for before x is staged: both latencies at once)
-        const int here = min(KC, a.K - kb);
-        for (int e = tid; e < here * RM; e += 512) {
-            const int r = e / here, k = e - r * here;
-            const int64_t row = row0 + r;
-            float x = 0.f;
-            if (row < a.M) {
-                if constexpr (sizeof(T) == 4) x = X[row * a.ldx + kb + k];
-                else x = __uint_as_float((uint32_t)X[row * a.ldx + kb + k] << 16);
+        const int here = min(KC, a.K - kb), staged = min(KC, (here + U * KS - 1) / (U * KS) * (U * KS));
+        for (int k = tid; k < staged; k += 512) {
+#pragma unroll
+            for (int r = 0; r < RM; ++r) {
+                const int64_t row = row0 + r;
+                float x = 0.f;
+                if (row < a.M && k < here) {
+                    if constexpr (sizeof(T) == 4) x = X[row * a.ldx + kb + k];
+                    else x = __uint_as_float((uint32_t)X[row * a.ldx + kb + k] << 16);
+                }
+                lds[k * RM + r] = x;
             }
-            lds[k * RM + r] = x;
         }
-        for (int e = here * RM + tid; e < KC * RM; e += 512) lds[e] = 0.f;
         __syncthreads();
         for (int it = 0; it * KS < here; it += U) {
             if (it) fetch(it);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float* x = lds + ((it + u) * KS + ks) * RM;
+                const int k = (it + u) * KS + ks;
+                const float* x = lds + k * RM;
+                float g[VEC], w[VEC];
+                values_of(wg[u], g);
+                values_of(wu[u], w);
+                if (it * KS + U * KS > here) {               // (a step that reaches behind the last row: zeros, whatever that row holds)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) { g[v] = k < here ? g[v] : 0.f; w[v] = k < here ? w[v] : 0.f; }
+                }
 #pragma unroll
                 for (int r = 0; r < RM; ++r)
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        acc[0][r][v] = fmaf(x[r], wg[u][v], acc[0][r][v]);
-                        acc[1][r][v] = fmaf(x[r], wu[u][v], acc[1][r][v]);
+                        acc[0][r][v] = fmaf(x[r], g[v], acc[0][r][v]);
+                        acc[1][r][v] = fmaf(x[r], w[v], acc[1][r][v]);
                     }
             }
         }
@@ -743,22 +773,28 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn
     }
 }
 
-// column sums of the partials: 64 columns a block, its four waves take every fourth part each (grid.y: dbg, dbu)
-__global__ __launch_bounds__(256) void bias_sum_kernel(const float* __restrict__ part, int nparts, int64_t part_ld, int N, float* __restrict__ d0, float* __restrict__ d1) {
-    __shared__ float red[4][64];
+// column sums of the partials: 64 columns a block, its 16 waves take every 16th part each, four at a time (grid.y: dbg, dbu)
+__global__ __launch_bounds__(1024) void bias_sum_kernel(const float* __restrict__ part, int nparts, int64_t part_ld, int N, float* __restrict__ d0, float* __restrict__ d1) {
+    __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < N) {
         const float* p = part + (int64_t)blockIdx.y * nparts * part_ld + c;
         int i = w;
-        for (; i + 12 < nparts; i += 16) {
-            s0 += p[(int64_t)i * part_ld]; s1 += p[(int64_t)(i + 4) * part_ld]; s2 += p[(int64_t)(i + 8) * part_ld]; s3 += p[(int64_t)(i + 12) * part_ld];
+        for (; i + 48 < nparts; i += 64) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[u] += p[(int64_t)(i + 16 * u) * part_ld];
         }
-        for (; i < nparts; i += 4) s0 += p[(int64_t)i * part_ld];
+        for (; i < nparts; i += 16) s[0] += p[(int64_t)i * part_ld];
     }
-    red[w][lane] = (s0 + s1) + (s2 + s3);
+    red[w][lane] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (w == 0 && c < N) (blockIdx.y ? d1 : d0)[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    if (w == 0 && c < N) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += red[i][lane];
+        (blockIdx.y ? d1 : d0)[c] = t;
+    }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------------------
@@ -1047,7 +1083,7 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
         hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, rows, part, part_ld);
         GEOGCN_LAUNCH_CHECK("gate_grad_kernel");
         if (part) {
-            hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)cdiv(b.N, 64), 2), dim3(256), 0, st, part, (int)nparts, part_ld, (int)b.N, b.db[0], b.db[1]);
+            hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)cdiv(b.N, 64), 2), dim3(1024), 0, st, part, (int)nparts, part_ld, (int)b.N, b.db[0], b.db[1]);
             GEOGCN_LAUNCH_CHECK("bias_sum_kernel");
         }
     }
