@@ -26,6 +26,7 @@ struct GemmCall {
     const float* gateG = nullptr; int64_t ldg = 0; const float* gateT = nullptr; int64_t ldt = 0;      // whole-rows kernels only
     const float* postY = nullptr; int64_t ldy = 0; const uint8_t* postKeep = nullptr; int64_t postF = 0; float postScale = 0.f;
     int precision = GEOGCN_GEMM_F32;         // GEOGCN_GEMM_F32 (exact) or GEOGCN_GEMM_BF16X3 (fp32-class split-bf16 where a kernel takes the shape)
+    float* gluH = nullptr; int64_t ldgluH = 0; int glu_act = 0;      // x3 whole-rows dual launches only: the gated block's H = act(C[0]) * C[1]; C[1] may be null (not kept)
     int64_t maxN() const { return n_nseg == 2 ? std::max(N[0], N[1]) : N[0]; }
 };
 

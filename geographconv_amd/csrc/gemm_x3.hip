@@ -20,6 +20,7 @@
 // Both run at the socket's power cap (1.4 kW, shader clock ~1.97 GHz: profiles/r05_x3_rows_clocks.txt): what they save is energy per
 // product as much as pipe time.
 #include "common.h"
+#include "gate.h"
 #include "gemm_call.h"
 
 #include <algorithm>
@@ -101,10 +102,13 @@ struct X3RowsArgs {
     int accumulate;
     const float* gateG; int64_t ldg; const float* gateT; int64_t ldt;                              // as RowsArgs (gemm.hip)
     const float* postY; int64_t ldy; const uint8_t* postKeep; int64_t postF; float postScale;
+    float* gluH; int64_t ldgluH; int glu_act;                       // GLU: dual launches of the gated dense block
     int panel_w; int64_t panel_R;       // single products only: C[0] as feature panels [N / panel_w][panel_R][panel_w] (the all-to-all's send layout, gemm.hip)
 };
 
-template <int KC, int ACT, bool GATE = false, bool POST = false>
+// GLU: the gated dense block H = act(G) * U on a dual launch's two products G (segment 0) and U (segment 1).  A wave takes the same columns of
+// both segments, all passes of segment 0 first: it stores G, and in segment 1's epilogue every lane reads back the G values it wrote itself.
+template <int KC, int ACT, bool GATE = false, bool POST = false, bool GLU = false>
 __global__ __launch_bounds__(TPB, 2) void x3_rows_kernel(const X3RowsArgs a) {
     constexpr int BM = kBM, WCT = kWCT, MR = BM / 16;
     constexpr int PITCH = KC * 2 + 16;           // bytes per LDS row and plane: an odd multiple of 16 -> conflict-free ds_read_b128
@@ -235,10 +239,10 @@ __global__ __launch_bounds__(TPB, 2) void x3_rows_kernel(const X3RowsArgs a) {
             const float* const gG = GATE ? a.gateG : nullptr; const float* const gT = GATE ? a.gateT : nullptr;
             const int64_t ldg = a.ldg, ldt = a.ldt, Mrows = a.M;
             const bool accum = a.accumulate != 0;
-            const bool extra = accum || gG != nullptr;
+            const bool extra = GLU ? seg == 1 : accum || gG != nullptr;
             f32x4 ea[WCT], eb[WCT];
-            const int64_t lda_e = gG ? ldg : ldc;
-            const __amdgpu_buffer_rsrc_t ersA = mk_rsrc((gG ? gG + m0 * ldg : Cout + m0 * ldc), extra ? rows_here * lda_e * 4 : 0);
+            const int64_t lda_e = GLU ? a.ldc[0] : gG ? ldg : ldc;
+            const __amdgpu_buffer_rsrc_t ersA = mk_rsrc(GLU ? a.C[0] + m0 * lda_e : (gG ? gG + m0 * ldg : Cout + m0 * ldc), extra ? rows_here * lda_e * 4 : 0);
             const __amdgpu_buffer_rsrc_t ersB = mk_rsrc(gG ? gT + m0 * ldt : Cout, gG ? rows_here * ldt * 4 : 0);
             const uint32_t lda_e4 = (uint32_t)lda_e * 4u, ldt4 = (uint32_t)ldt * 4u;
             const __amdgpu_buffer_rsrc_t prsY = mk_rsrc(POST ? a.postY + m0 * a.ldy : Cout, POST ? rows_here * a.ldy * 4 : 0);
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(TPB, 2) void x3_rows_kernel(const X3RowsArgs a) {
                         x[r] = acc[i][j][r] + bcol[j][r];
                         if (ACT == GEOGCN_ACT_NONE || act_on) x[r] = apply_act<ACT>(x[r]);
                     }
-                    if (accum) { x[0] += ea[j][0]; x[1] += ea[j][1]; x[2] += ea[j][2]; x[3] += ea[j][3]; }
+                    if (!GLU && accum) { x[0] += ea[j][0]; x[1] += ea[j][1]; x[2] += ea[j][2]; x[3] += ea[j][3]; }
                     if constexpr (GATE) {
                         f32x4 tq;
                         if constexpr (POST) tq = pt;
@@ -301,9 +305,17 @@ __global__ __launch_bounds__(TPB, 2) void x3_rows_kernel(const X3RowsArgs a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (col0 + r >= Nseg) x[r] = 0.f;
-                    if (row_ok && col0 < Nseg) {
+                    if constexpr (GLU) {
+                        if (seg == 1 && row_ok && col0 < Nseg) {
+                            float h[4];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) h[r] = col0 + r < Nseg ? gate_value(a.glu_act, ea[j][r]) * x[r] : 0.f;
+                            *reinterpret_cast<float4*>(a.gluH + row * a.ldgluH + col0) = make_float4(h[0], h[1], h[2], h[3]);
+                        }
+                    }
+                    if (row_ok && col0 < Nseg && (!GLU || Cout)) {
                         float* dst = crow + col0;
-                        if constexpr (!GATE && !POST) {
+                        if constexpr (!GATE && !POST && !GLU) {
                             if (a.panel_w) {          // (panel_w % 4 == 0: the four columns of a lane lie in one panel)
                                 const int64_t q = col0 / a.panel_w;
                                 dst = Cout + (q * a.panel_R + row) * a.panel_w + (col0 - q * a.panel_w);
@@ -467,7 +479,8 @@ int launch_x3_rows(const X3RowsArgs& a, int act, hipStream_t st) {
         hipLaunchKernelGGL(kern, dim3((unsigned)G), dim3(TPB), lds, st, a);                                      \
         GEOGCN_LAUNCH_CHECK("x3_rows_kernel");                                                                   \
     } while (0)
-    if (a.gateG && a.postY) GEOGCN_XR(GEOGCN_ACT_NONE, true, true);
+    if (a.gluH) GEOGCN_XR(GEOGCN_ACT_NONE, false, false, true);
+    else if (a.gateG && a.postY) GEOGCN_XR(GEOGCN_ACT_NONE, true, true);
     else if (a.gateG) GEOGCN_XR(GEOGCN_ACT_NONE, true);
     else if (act == GEOGCN_ACT_TANH) GEOGCN_XR(GEOGCN_ACT_TANH);
     else if (act == GEOGCN_ACT_SIGMOID) GEOGCN_XR(GEOGCN_ACT_SIGMOID);
@@ -521,6 +534,7 @@ int x3_run_rows(int kc, bool transB, const GemmCall& c, void* ws, hipStream_t st
     a.gateG = c.gateG; a.ldg = c.ldg; a.gateT = c.gateT; a.ldt = c.ldt;
     a.postY = c.postY; a.ldy = c.ldy; a.postKeep = c.postKeep; a.postF = c.postF; a.postScale = c.postScale;
     a.panel_w = c.panel_w; a.panel_R = c.panel_R;
+    a.gluH = c.gluH; a.ldgluH = c.ldgluH; a.glu_act = c.glu_act;
     const int ks = kc / 32;
     for (int q = 0; q < 2; ++q) {
         a.A[q] = c.A[q]; a.lda[q] = c.lda[q]; a.K[q] = (int)c.K[q];

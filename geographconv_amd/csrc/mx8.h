@@ -58,14 +58,17 @@ __device__ __forceinline__ void bf16_terms4(const float4& x, uint2 (&t)[P]) {
 // four consecutive values of row r from column c (c % 4 == 0, c < roundup4(F) <= ld) of a matrix of one of the three storage types; columns
 // from F on read as zero whatever the pad holds
 struct MatIn { int type; const void* p; int64_t ld; const uint8_t* scale; };
-__device__ __forceinline__ float4 mat_load4_raw(const MatIn& m, int64_t r, int c) {
-    if (m.type == GEOGCN_T_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(m.p) + r * m.ld + c);
-    if (m.type == GEOGCN_T_BF16) {
+template <int TYPE>
+__device__ __forceinline__ float4 mat_load4(const MatIn& m, int64_t r, int c) {
+    if constexpr (TYPE == GEOGCN_T_F32) {
+        return *reinterpret_cast<const float4*>(static_cast<const float*>(m.p) + r * m.ld + c);
+    } else if constexpr (TYPE == GEOGCN_T_BF16) {
         const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(m.p) + r * m.ld + c);
         return make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(m.p) + r * m.ld + c);
+        return mx8_decode4(w, mx8_scale(m.scale[r * (m.ld / kMxBlock) + c / kMxBlock]));
     }
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(m.p) + r * m.ld + c);
-    return mx8_decode4(w, mx8_scale(m.scale[r * (m.ld / kMxBlock) + c / kMxBlock]));
 }
 __device__ __forceinline__ float4 mask4(float4 v, int c, int F) {
     if (c + 3 >= F) {

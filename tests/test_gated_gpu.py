@@ -83,7 +83,7 @@ def _check(got, ref, what):
 
 FORWARD = [(1, 1, 1), (1, 300, 300), (1, 1024, 513), (2, 64, 32), (3, 33, 65), (7, 300, 930), (8, 129, 256), (9, 40, 7), (17, 1000, 31), (31, 2048, 40),
            (33, 7, 300), (64, 512, 96), (65, 100, 129), (128, 128, 128), (129, 300, 600), (200, 930, 517), (257, 65, 320), (700, 96, 161), (4500, 300, 300),
-           (1000, 640, 1300)]
+           (1000, 640, 1300), (16400, 300, 300), (16385, 600, 257), (17001, 40, 640), (16384, 200, 129)]
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16'])
@@ -110,7 +110,7 @@ def test_forward(dev, M, K, N, dtype):
         half = np.maximum(2.0 ** -4 * (np.abs(want) + bound), 2.0 ** -10 * s)
         out16 = BF * np.abs(want) if dtype == 'bf16' else 0
         _check(got, (want, half * (1 + 1e-6) + bound + out16), 'checkpoint')
-        if dtype == 'f32':                               # ... and they are the codes of the very values the other form keeps
+        if dtype == 'f32' and M < 16384:                 # ... and they are the codes of the very values the other form keeps (one kernel forms both)
             p = ops.mx8_pack(kept.G if q is k8.G else kept.U)
             assert torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
 
@@ -147,7 +147,7 @@ def test_saturated_gates(dev):
 
 
 BACKWARD = [(1, 1, 1), (1, 300, 300), (2, 33, 65), (5, 64, 64), (31, 129, 40), (64, 300, 33), (130, 40, 300), (300, 257, 129), (1000, 300, 930), (5000, 96, 161),
-            (4200, 300, 300), (700, 1100, 200)]
+            (4200, 300, 300), (700, 1100, 200), (16390, 300, 200), (16385, 129, 300), (17000, 400, 70)]
 
 
 def _check_bwd(dev, d, r, dH, kept, name, dtype, X=None, precision=None, need_dx=True, bias=True):
