@@ -614,8 +614,17 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         for (int q = 0; q < 2; ++q) {
             if (q >= a.nseg) break;
             const float* w = a.W + row * a.ldw + q * a.segw + col;
-            for (int z = 0; z < a.nsplit; ++z) {
-                const float4 t = *reinterpret_cast<const float4*>(w + (int64_t)z * a.M * a.ldw);
+            const int64_t zs = a.M * a.ldw;
+            int z = 0;
+            for (; z + 8 <= a.nsplit; z += 8) {               // eight loads in flight, added in order
+                float4 t[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) t[u] = *reinterpret_cast<const float4*>(w + (z + u) * zs);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) { v[q][0] += t[u].x; v[q][1] += t[u].y; v[q][2] += t[u].z; v[q][3] += t[u].w; }
+            }
+            for (; z < a.nsplit; ++z) {
+                const float4 t = *reinterpret_cast<const float4*>(w + z * zs);
                 v[q][0] += t.x; v[q][1] += t.y; v[q][2] += t.z; v[q][3] += t.w;
             }
         }
@@ -655,13 +664,14 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
 }
 
 // ---- dG, dU as term planes (P = 0: as fp32 matrices), with the partial column sums of both (bias gradients) ------------------------------
-// A block takes `rows` rows of 256 columns; its partial sums are rows / 4 sequential adds per wave, then a tree.
+// A block takes `rows` rows of qw * 4 columns; its partial sums are rows / rw sequential adds per thread, then rw.
 template <int P, int TD, int TK>
 __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn U, int64_t M, int N, int act, uint16_t* __restrict__ oG,
-                                                        uint16_t* __restrict__ oU, int cols, int64_t ldo, int64_t plane, int rows, float* __restrict__ part, int64_t part_ld) {
-    __shared__ float red[4][64][8];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int c = (blockIdx.x * 64 + lane) * 4;
+                                                        uint16_t* __restrict__ oU, int cols, int64_t ldo, int64_t plane, int rows, int qw, float* __restrict__ part, int64_t part_ld) {
+    __shared__ float red[256][8];
+    // qw quads of columns side by side, rw = 256 / qw rows at a time (300 columns: 75 x 3, not 64 of one block and 11 of the next)
+    const int w = threadIdx.x / qw, lane = threadIdx.x - w * qw, rw = 256 / qw;
+    const int c = w < rw ? (blockIdx.x * qw + lane) * 4 : cols;
     const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = min(M, r0 + rows);
     const int cc = c < N ? c : 0;                             // (a lane of pad columns reads the first ones and writes zeros)
     float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
@@ -694,23 +704,25 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn
             }
         };
         int64_t r = r0 + w;
-        for (; r + 4 < r1; r += 8) {                          // two rows' loads in flight
+        for (; r + rw < r1; r += 2 * rw) {                    // two rows' loads in flight
             const float4 d0 = mat_load4<TD>(dH, r, cc), g0 = mat_load4<TK>(G, r, cc), u0 = mat_load4<TK>(U, r, cc);
-            const float4 d1 = mat_load4<TD>(dH, r + 4, cc), g1 = mat_load4<TK>(G, r + 4, cc), u1 = mat_load4<TK>(U, r + 4, cc);
+            const float4 d1 = mat_load4<TD>(dH, r + rw, cc), g1 = mat_load4<TK>(G, r + rw, cc), u1 = mat_load4<TK>(U, r + rw, cc);
             one(r, d0, g0, u0);
-            one(r + 4, d1, g1, u1);
+            one(r + rw, d1, g1, u1);
         }
         if (r < r1) one(r, mat_load4<TD>(dH, r, cc), mat_load4<TK>(G, r, cc), mat_load4<TK>(U, r, cc));
     }
     if (!part) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { red[w][lane][k] = sg[k]; red[w][lane][4 + k] = su[k]; }
+    for (int k = 0; k < 4; ++k) { red[threadIdx.x][k] = sg[k]; red[threadIdx.x][4 + k] = su[k]; }
     __syncthreads();
-    if (w < 2 && c < N) {
-        float s[4];
+    if (w == 0 && c < N) {
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < rw; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] = (red[0][lane][w * 4 + k] + red[1][lane][w * 4 + k]) + (red[2][lane][w * 4 + k] + red[3][lane][w * 4 + k]);
-        *reinterpret_cast<float4*>(part + ((int64_t)w * gridDim.y + blockIdx.y) * part_ld + c) = make_float4(s[0], s[1], s[2], s[3]);
+            for (int k = 0; k < 8; ++k) s[k] += red[i * qw + lane][k];
+        *reinterpret_cast<float4*>(part + (int64_t)blockIdx.y * part_ld + c) = make_float4(s[0], s[1], s[2], s[3]);
+        *reinterpret_cast<float4*>(part + ((int64_t)gridDim.y + blockIdx.y) * part_ld + c) = make_float4(s[4], s[5], s[6], s[7]);
     }
 }
 
@@ -980,11 +992,13 @@ int forward_exact(Arena& ar, const FwdArgs& f, hipStream_t st) {
     return finish(t, 2, EPI_GATED, st);
 }
 // fp32 blocks of many rows: the library's whole-rows kernel reads X as it is (no term planes in memory) and takes all columns of 64 rows.
-// It starts at 16,384 rows, where its 64-row blocks go round the CUs (440,000 x 300 -> 300 with G, U kept: 1,598 us by tiles; 20,000 x 300:
-// 92; 9,475 x 300 -> 600: 81 by tiles against 80 for the plain products alone), and not for kept checkpoints, whose blocks its waves share.
+// It starts at 16,384 rows, where its 64-row blocks go round the CUs -- 32,768 where either width passes 640 and a block works longer --, and
+// not for kept checkpoints, whose blocks its waves share.  By tiles / by whole rows, G and U kept: 440,000 x 300 -> 300 1,598 / 1,156 us,
+// 20,000 x 300 -> 300 92 / 80, 60,000 x 600 -> 600 628 / 566, 20,000 x 900 -> 930 449 / 523, 60,000 x 900 -> 900 1,243 / 1,169.
 constexpr int64_t kWholeRowsMin = 16384;
 int whole_rows(const FwdArgs& f, GemmCall* c) {
-    if (f.type != GEOGCN_T_F32 || f.precision != GEOGCN_GEMM_BF16X3 || f.keep == GEOGCN_KEEP_MX8 || f.M < kWholeRowsMin || f.K == 0) return 0;
+    if (f.type != GEOGCN_T_F32 || f.precision != GEOGCN_GEMM_BF16X3 || f.keep == GEOGCN_KEEP_MX8 || f.K == 0) return 0;
+    if (f.M < (std::max(f.K, f.N) > 640 ? 2 * kWholeRowsMin : kWholeRowsMin)) return 0;
     *c = GemmCall{};
     c->M = f.M; c->n_nseg = 2; c->n_kseg = 1; c->precision = GEOGCN_GEMM_BF16X3;
     c->A[0] = static_cast<const float*>(f.X.p); c->lda[0] = f.X.ld; c->K[0] = f.K;
@@ -1035,10 +1049,12 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
     const int64_t ldt = P ? P * ldo : ldo, plane = ldo, bytes = b.M * ldt * (P ? 2 : 4);
     uint16_t* dG = *dG_out = static_cast<uint16_t*>(ar.take(bytes));
     uint16_t* dU = *dU_out = static_cast<uint16_t*>(ar.take(bytes));
-    // rows of a block: enough blocks to keep every CU at eight, and 1,024 rows where they are long anyway
-    const int64_t cblocks = cdiv(ldo, 256);
-    const int rows = (int)std::max(std::min<int64_t>(1024, std::max<int64_t>(4, up(cdiv(b.M * cblocks, (int64_t)kNumCU * 8), 4))),
-                                   up(cdiv(b.M, 65535), 4));          // (grid.y)
+    // quads of columns of a block: all of them, or equal shares where there are more than 256; rows: enough blocks to keep every CU at eight, and
+    // 1,024 rows where they are long anyway
+    const int64_t quads = cdiv(ldo, 4), cblocks = cdiv(quads, 256);
+    const int qw = (int)cdiv(quads, cblocks), rw = 256 / qw;
+    const int rows = (int)std::max(std::min<int64_t>(1024, std::max<int64_t>(2 * rw, up(cdiv(b.M * cblocks, (int64_t)kNumCU * 8), 2 * rw))),
+                                   up(cdiv(b.M, 65535), 2 * rw));     // (grid.y)
     const int64_t nparts = cdiv(b.M, rows), part_ld = up(b.N, 4);
     float* part = b.db[0] ? static_cast<float*>(ar.take(2 * nparts * part_ld * 4)) : nullptr;
     if (!ar.counting) {
@@ -1049,7 +1065,7 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
                   : P == 3 ? (q8 ? &gate_grad_kernel<3, F, Q> : &gate_grad_kernel<3, F, F>)
                   : P == 1 ? (q8 ? &gate_grad_kernel<1, F, Q> : &gate_grad_kernel<1, F, F>)
                            : (q8 ? &gate_grad_kernel<0, F, Q> : &gate_grad_kernel<0, F, F>);
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, rows, part, part_ld);
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, b.dH, b.G, b.U, b.M, (int)b.N, b.act, dG, dU, (int)ldo, ldt, plane, rows, qw, part, part_ld);
         GEOGCN_LAUNCH_CHECK("gate_grad_kernel");
         if (part) {
             hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)cdiv(b.N, 64), 2), dim3(1024), 0, st, part, (int)nparts, part_ld, (int)b.N, b.db[0], b.db[1]);
@@ -1057,6 +1073,31 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
         }
     }
     return 0;
+}
+// X^T.[B0 | B1] of a checkpointed X and fp32 matrices by the library's A^T.B kernel: X's codes and the fp32 values are read as they are
+bool tn_q8_takes(int64_t M, int64_t K, int64_t N) { return M >= kWholeRowsMin && K <= 320 && N <= 1024; }
+int tn_q8(Arena& ar, const MatIn& X, int64_t M, int64_t K, int64_t N, int nseg, const float* const* B, int64_t ldb, void* const* dW, const int64_t* lddw,
+          hipStream_t st) {
+    const int bn = up(N, 256) <= up(N, 320) ? 256 : 320;
+    X3TnCall t{};
+    t.M = K; t.K = M; t.A8 = static_cast<const uint8_t*>(X.p); t.S8 = X.scale; t.ld8 = X.ld;
+    t.n_mt = (int)cdiv(K, 160); t.nt_per_seg = (int)cdiv(N, bn); t.n_nt = nseg * t.nt_per_seg;
+    // one block a CU and the tiles of a slab on one XCD: as many whole slabs as its 32 CUs take
+    const int T = t.n_mt * t.n_nt;
+    t.kchunk = up(cdiv(M, (int64_t)kNumXCD * std::max(1, kNumCU / kNumXCD / T)), 32);
+    t.nsplit = (int)cdiv(M, t.kchunk);
+    t.seg_w = up(N, kMxBlock); t.ldw = nseg * t.seg_w;
+    t.W = static_cast<float*>(ar.take((int64_t)t.nsplit * K * t.ldw * 4));
+    if (ar.counting) return 0;
+    TileArgs f = tile_args();
+    f.M = K; f.N = N; f.nsplit = t.nsplit; f.W = t.W; f.segw = t.seg_w; f.ldw = t.ldw; f.out_type = GEOGCN_T_F32;
+    f.ncols = up(N, 4);
+    for (int q = 0; q < nseg; ++q) {
+        t.B[q] = B[q]; t.ldb[q] = ldb; t.N[q] = N;
+        f.C[q] = dW[q]; f.ldc[q] = lddw[q];
+    }
+    if (const int rc = x3_tn_launch(160, bn, t, st)) return rc;
+    return finish(f, nseg, EPI_STORE, st);
 }
 // the products by the library's fp32 kernels: dG, dU (and a checkpointed X) as fp32 matrices
 int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
@@ -1072,7 +1113,10 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
                                                     static_cast<const float*>(b.Wu.p), b.Wu.ld, static_cast<float*>(b.dX), b.lddx, 0, precision,
                                                     need ? w : nullptr, need, st)) return rc;
     }
-    if (b.dW[0]) {
+    if (b.dW[0] && precision == GEOGCN_GEMM_BF16X3 && b.X.type == GEOGCN_T_MX8) {
+        const float* B[2] = {dG, dU};
+        if (const int rc = tn_q8(ar, b.X, b.M, b.K, b.N, 2, B, ldo, b.dW, b.lddw, st)) return rc;
+    } else if (b.dW[0]) {
         const float* X = static_cast<const float*>(b.X.p);
         int64_t ldx = b.X.ld;
         if (b.X.type == GEOGCN_T_MX8) {
@@ -1096,7 +1140,7 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
     // fp32 over many rows and up to 320 inputs (one tile of the library's A^T.B kernel): dG, dU stay fp32 matrices and the library's split-bf16
     // kernels multiply them (440,000 x 300 -> 300: 2.17 + 0.92 ms by tiles, against 0.86 + 1.07 ms and a gate pass of 0.55; 60,000 x 600 ->
     // 600: 1.14 against 1.40)
-    if (b.type == GEOGCN_T_F32 && b.X.type == GEOGCN_T_F32 && b.precision == GEOGCN_GEMM_BF16X3 && b.M >= kWholeRowsMin && b.K <= 320 && b.N <= 1024)
+    if (b.type == GEOGCN_T_F32 && b.precision == GEOGCN_GEMM_BF16X3 && tn_q8_takes(b.M, b.K, b.N))
         return backward_exact(ar, b, GEOGCN_GEMM_BF16X3, st);
     const int P = terms_of(b.type, b.precision), PX = b.X.type == GEOGCN_T_F32 ? P : 1;
     const int64_t plane = up(b.N, 64), ldo = P * plane;
@@ -1144,6 +1188,10 @@ int weight_grad_exact(Arena& ar, const WgradArgs& w, hipStream_t st) {
 }
 int weight_grad(Arena& ar, const WgradArgs& w, hipStream_t st) {
     if (w.precision == GEOGCN_GEMM_F32 && w.type == GEOGCN_T_F32) return weight_grad_exact(ar, w, st);
+    if (w.type == GEOGCN_T_F32 && w.precision == GEOGCN_GEMM_BF16X3 && tn_q8_takes(w.M, w.K, w.N)) {
+        const float* B[1] = {static_cast<const float*>(w.dZ.p)};
+        return tn_q8(ar, w.X, w.M, w.K, w.N, 1, B, w.dZ.ld, &w.dW, &w.lddw, st);
+    }
     const int P = terms_of(w.type, w.precision);
     Planes x, dz;
     if (const int rc = make_planes(ar, w.X, w.M, w.K, 1, false, st, &x)) return rc;

@@ -44,6 +44,7 @@ struct X3TnCall {
     float* W; int64_t ldw, seg_w;       // slabs [nsplit][M][ldw]; N segment q starts at column q * seg_w
     int n_mt, n_nt, nt_per_seg, nsplit;
     int64_t kchunk;                     // a multiple of 32
+    const uint8_t* A8 = nullptr; const uint8_t* S8 = nullptr; int64_t ld8 = 0;      // A as an 8-bit checkpoint (codes, scales, code pitch) instead; tiles 160 x 320, 160 x 256
 };
 int x3_tn_launch(int bm, int bn, const X3TnCall& t, hipStream_t st);
 

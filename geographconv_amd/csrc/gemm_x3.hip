@@ -22,6 +22,7 @@
 #include "common.h"
 #include "gate.h"
 #include "gemm_call.h"
+#include "mx8.h"
 
 #include <algorithm>
 
@@ -337,7 +338,9 @@ __global__ __launch_bounds__(TPB, 2) void x3_rows_kernel(const X3RowsArgs a) {
 // ---- A^T . B ----------------------------------------------------------------------------------------------------------------------------
 constexpr int BKH = 32, ROWB = 80;      // k per stage = one MFMA depth; bytes per LDS row: 32 bf16 + 16 B pad (an odd multiple of 16)
 
-template <int BM, int BN>
+// Q8: A is an 8-bit checkpoint (mx8.h).  Its values are one bf16 term each, read as codes (a dword a row of the patch) and scale bytes: three
+// products instead of six, one image of A instead of three.
+template <int BM, int BN, bool Q8 = false>
 __global__ __launch_bounds__(512, 1) void x3_tn_kernel(const X3TnCall a) {
     constexpr int NTH = 512, kASplit = 192;                  // threads [0,192): A patches, [192,512): B patches
     constexpr int MR = BM / 32, NR = BN / 64;                // 2 x 4 waves, wave tile (BM/2) x (BN/4)
@@ -379,6 +382,20 @@ __global__ __launch_bounds__(512, 1) void x3_tn_kernel(const X3TnCall a) {
     f32x4 patch[8];
     auto gload = [&](int kt) {
         const int64_t k0 = kbeg + (int64_t)kt * BKH;
+        if constexpr (Q8) {
+            if (isA) {                      // component 0: four codes, component 1: their block's scale byte (rows past the end: code 0, scale 0)
+                const int64_t lds8 = a.ld8 / kMxBlock;
+                const __amdgpu_buffer_rsrc_t rc = mk_rsrc(a.A8 + k0 * a.ld8 + c0, (kend - k0) * a.ld8 - c0);
+                const __amdgpu_buffer_rsrc_t rb = mk_rsrc(a.S8 + k0 * lds8 + c0 / kMxBlock, (kend - k0) * lds8 - c0 / kMxBlock);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t row = (uint32_t)(k8 * 8 + i);
+                    patch[i][0] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rc, (int)(col_ok ? row * (uint32_t)a.ld8 + (uint32_t)c4 * 4u : kOob), 0, 0));
+                    patch[i][1] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rb, (int)(col_ok ? row * (uint32_t)lds8 + (uint32_t)c4 / 8u : kOob), 0, 0));
+                }
+                return;
+            }
+        }
         // the descriptor ends with the slab: rows past it (and stages past the slab) read as zeros in hardware
         const __amdgpu_buffer_rsrc_t rs = mk_rsrc(Pp + k0 * ld + c0, ((kend - k0) * ld - c0) * 4);
         const uint32_t ld4 = (uint32_t)ld * 4u;
@@ -390,6 +407,21 @@ __global__ __launch_bounds__(512, 1) void x3_tn_kernel(const X3TnCall a) {
     auto sstore = [&]() {
         if (!active) return;
         unsigned char* img = smem_raw + (isA ? 0 : kImgA);
+        if constexpr (Q8) {
+            if (isA) {
+                float v[8][4];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float4 x = mx8_decode4(__float_as_uint(patch[i][0]), mx8_scale(__float_as_uint(patch[i][1])));
+                    v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<uint4*>(img + (c4 * 4 + e) * ROWB + k8 * 16) =
+                        make_uint4(bf16_pack(v[0][e], v[1][e]), bf16_pack(v[2][e], v[3][e]), bf16_pack(v[4][e], v[5][e]), bf16_pack(v[6][e], v[7][e]));
+                return;
+            }
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             uint32_t p[4][3];
@@ -417,11 +449,12 @@ __global__ __launch_bounds__(512, 1) void x3_tn_kernel(const X3TnCall a) {
         __syncthreads();
         const unsigned char* Asm = smem_raw;
         const unsigned char* Bsm = smem_raw + kImgA;
-        bf16x8 af[MR][3];
+        constexpr int PA = Q8 ? 1 : 3;
+        bf16x8 af[MR][PA];
 #pragma unroll
         for (int i = 0; i < MR; ++i)
 #pragma unroll
-            for (int pl = 0; pl < 3; ++pl)
+            for (int pl = 0; pl < PA; ++pl)
                 af[i][pl] = *reinterpret_cast<const bf16x8*>(Asm + pl * kPlane + (wm * (BM / 2) + i * 16 + li) * ROWB + lg * 16);
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
@@ -431,7 +464,11 @@ __global__ __launch_bounds__(512, 1) void x3_tn_kernel(const X3TnCall a) {
                 bf[pl] = *reinterpret_cast<const bf16x8*>(Bsm + pl * kPlane + (wn * (BN / 4) + j * 16 + li) * ROWB + lg * 16);
 #define GEOGCN_ACC_(i_) acc[i_][j]
 #define GEOGCN_AF_(i_) af[i_]
-            GEOGCN_X3_SIX(GEOGCN_ACC_, bf, GEOGCN_AF_, MR)
+            if constexpr (Q8) {
+                GEOGCN_X3_TERM(GEOGCN_ACC_, bf, GEOGCN_AF_, 2, 0, MR) GEOGCN_X3_TERM(GEOGCN_ACC_, bf, GEOGCN_AF_, 1, 0, MR) GEOGCN_X3_TERM(GEOGCN_ACC_, bf, GEOGCN_AF_, 0, 0, MR)
+            } else {
+                GEOGCN_X3_SIX(GEOGCN_ACC_, bf, GEOGCN_AF_, MR)
+            }
 #undef GEOGCN_ACC_
 #undef GEOGCN_AF_
         }
@@ -577,16 +614,21 @@ bool x3_tn_takes(int bm, int bn) {
 int x3_tn_launch(int bm, int bn, const X3TnCall& t, hipStream_t st) {
     const int T = t.n_mt * t.n_nt;
     const dim3 grid((unsigned)(cdiv(t.nsplit, kNumXCD) * kNumXCD * T));
-#define GEOGCN_XT(BM_, BN_)                                                                                      \
+#define GEOGCN_XT(BM_, BN_, ...)                                                                                      \
     do {                                                                                                         \
-        auto kern = x3_tn_kernel<BM_, BN_>;                                                                      \
+        auto kern = x3_tn_kernel<BM_, BN_, ##__VA_ARGS__>;                                                                      \
         constexpr int lds = 3 * (BM_ + BN_) * ROWB;                                                              \
         static LdsAttrOnce lds_once;                                                                           \
         if (const int rc_ = lds_once.ensure((const void*)kern, (int)(lds))) return rc_; \
         hipLaunchKernelGGL(kern, grid, dim3(512), lds, st, t);                                                   \
         GEOGCN_LAUNCH_CHECK("x3_tn_kernel");                                                                     \
     } while (0)
-    if (bm == 160 && bn == 320) GEOGCN_XT(160, 320);
+    if (t.A8 && bm == 160 && bn == 320) GEOGCN_XT(160, 320, true);
+    else if (t.A8 && bm == 160 && bn == 256) GEOGCN_XT(160, 256, true);
+    else if (t.A8) {
+        set_error("x3_tn_launch: no kernel for tile %dx%d of a checkpoint", bm, bn);
+        return GEOGCN_E_ARG;
+    } else if (bm == 160 && bn == 320) GEOGCN_XT(160, 320);
     else if (bm == 160 && bn == 256) GEOGCN_XT(160, 256);
     else if (bm == 128 && bn == 320) GEOGCN_XT(128, 320);
     else if (bm == 128 && bn == 256) GEOGCN_XT(128, 256);

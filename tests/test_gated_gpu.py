@@ -292,7 +292,7 @@ def test_checkpoint_format(dev, n, F, dtype):
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16'])
-@pytest.mark.parametrize('M,K,N', [(1, 1, 1), (3, 33, 5), (40, 300, 129), (129, 64, 64), (1000, 300, 256), (5000, 200, 300), (300, 700, 1000)])
+@pytest.mark.parametrize('M,K,N', [(1, 1, 1), (3, 33, 5), (40, 300, 129), (129, 64, 64), (1000, 300, 256), (5000, 200, 300), (300, 700, 1000), (16500, 300, 256), (20001, 33, 129), (16384, 320, 700)])
 def test_weight_gradient_from_a_checkpoint(dev, M, K, N, dtype):
     from geographconv_amd import ops
     x8 = ops.mx8_pack(_mat(_rand((M, K), 1), dev, dtype))
