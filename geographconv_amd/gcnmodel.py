@@ -328,6 +328,17 @@ def residual_dense(incoming, nonlinearity=NL.selu):
     return L.NonlinearityLayer(convX_plus_X, nonlinearity=nonlinearity)
 
 
+def gated_dense_block(incoming, num_hidden=None, nonlinearity=NL.swish, checkpoint=None, Wg=_init.GlorotUniform(), Wu=_init.GlorotUniform(),
+                      W=_init.GlorotUniform()):
+    """incoming + Dense(act(x . Wg) * (x . Wu)): a gated hidden layer of `num_hidden` units (default: twice the inputs), projected back and
+    added to its input -- a dense block to stand between convolutions, beside highway_dense and residual_dense (not in the reference).
+    `checkpoint='mx8'`: its activations wait for the backward in 8 bits."""
+    num_inputs = int(np.prod(incoming.output_shape[1:]))
+    hidden = L.GatedDenseLayer(incoming, num_hidden or 2 * num_inputs, Wg=Wg, Wu=Wu, nonlinearity=nonlinearity, checkpoint=checkpoint)
+    back = DenseLayer(hidden, num_units=num_inputs, W=W, nonlinearity=None, checkpoint=checkpoint)
+    return L.ElemwiseSumLayer([back, incoming], coeffs=1, cropping=None)
+
+
 def np_softmax(x):
     e_x = np.exp(x - np.max(x))
     return e_x / e_x.sum()

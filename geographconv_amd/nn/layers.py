@@ -237,16 +237,31 @@ def _accumulate(dst, src):
 # --------------------------------------------------------------------------------------------
 # dense / dropout (lasagne.layers.dense, lasagne.layers.noise)
 # --------------------------------------------------------------------------------------------
+def _check_checkpoint(checkpoint):
+    if checkpoint not in (None, 'mx8'):
+        raise ValueError("checkpoint is None or 'mx8', not %r" % (checkpoint,))
+    return checkpoint
+
+
+def _checkpointed(x):
+    """Is this a tape entry kept in 8 bits (ops.MX8Mat)?"""
+    return isinstance(x, getattr(backend.active(), 'MX8Mat', ()))
+
+
 class DenseLayer(Layer):
-    """y = nonlinearity(x . W + b)   (lasagne DenseLayer; the highway gate, gcnmodel.py:285)."""
+    """y = nonlinearity(x . W + b)   (lasagne DenseLayer; the highway gate, gcnmodel.py:285).
+
+    ``checkpoint='mx8'`` (dense input, outside the graph product): the tape keeps x in 8 bits (ops.mx8_pack, 1.03 bytes a value) and the
+    weight gradient is taken from the codes; the forward and the input gradient are unchanged."""
 
     early_starts = {'fwd': 0, 'bwd': 0}     # exchanges started ahead of their layer (diagnostics / tests)
 
     def __init__(self, incoming, num_units, W=_init.GlorotUniform(), b=_init.Constant(0.), nonlinearity=_nl.rectify,
-                 name=None, **kwargs):
+                 name=None, checkpoint=None, **kwargs):
         super().__init__(incoming, name)
         self.nonlinearity = _nl.resolve(nonlinearity)
         self.num_units = int(num_units)
+        self.checkpoint = _check_checkpoint(checkpoint)
         num_inputs = int(np.prod(self.input_shape[1:]))
         self.W = self.add_param(W, (num_inputs, self.num_units), name="W")
         self.b = None if b is None else self.add_param(b, (self.num_units,), name="b", regularizable=False)
@@ -284,6 +299,11 @@ class DenseLayer(Layer):
         A = kwargs.get('A') if self._uses_graph(kwargs) else None
         prec = kwargs.get('gemm_precision')     # None = backend default (tuning.GEMM_PRECISION: 'bf16x3'; 'f32' = exact fp32 MFMA)
         saved = {'x': input}
+        if self.checkpoint is not None:
+            if A is not None or not isinstance(input, K.DMat) or hasattr(self, 'highway_conv') or hasattr(self, 'highway_gate'):
+                raise ValueError("checkpoint: a dense layer with a dense input outside the graph product and the highway block")
+            if tape is not None:
+                saved['x'] = K.mx8_pack(input)
         if A is None:
             conv = self._fusable_sibling(input, tape, kwargs)
             if conv is not None:
@@ -398,7 +418,7 @@ class DenseLayer(Layer):
         keep = tape.get(d, {}).get('mask')
         if (keep is None or not isinstance(below, DenseLayer) or below.nonlinearity is not _nl.tanh or below.b is None
                 or kwargs.get('consumers', {}).get(d) != 3 or kwargs.get('consumers', {}).get(below) != 1
-                or isinstance(tape.get(below, {}).get('x'), K.DMat)):
+                or isinstance(tape.get(below, {}).get('x'), K.DMat) or _checkpointed(tape.get(below, {}).get('x'))):
             return None
         y0 = tape[below]['y']
         # (an injected mask of another dtype / layout / device -- parity runs -- takes the unfused Masked / act_bwd path, which accepts it)
@@ -466,7 +486,7 @@ class DenseLayer(Layer):
             dS = grad
         else:
             # (dS is gathered row-wise by the next product -- A^T . dS, or X^T . dS0 under a sparse input: line-aligned pitch)
-            uses_graph = (self._uses_graph(kwargs) and kwargs.get('A') is not None) or not isinstance(tape[self]['x'], K.DMat)
+            uses_graph = (self._uses_graph(kwargs) and kwargs.get('A') is not None) or not (isinstance(tape[self]['x'], K.DMat) or _checkpointed(tape[self]['x']))
             km, sc = (grad.keep_mask, grad.scale) if isinstance(grad, Masked) else (None, 1.0)
             g_in = grad.m if isinstance(grad, Masked) else grad
             out = K.DMat.empty(g_in.n, g_in.F, g_in.device, ld=K.gather_ld(g_in.F)) if uses_graph else None
@@ -530,7 +550,7 @@ class DenseLayer(Layer):
     def _backward_post(self, x, dZ, into, need_input_grad, kwargs, tape=None):
         K = backend.active()
         lazy = into[0] if isinstance(into[0], K.GateCarry) else None
-        if isinstance(x, K.DMat):
+        if isinstance(x, K.DMat) or _checkpointed(x):
             prec = kwargs.get('gemm_precision')
             gate = getattr(self, 'highway_gate', None)
             if (tape is not None and gate is not None and tape.get(gate, {}).get('fused_with') is self
@@ -566,7 +586,10 @@ class DenseLayer(Layer):
                                     accumulate=into[0] is not None, precision=prec)]
             if lazy is not None and not need_input_grad:
                 lazy = None
-            K.gemm(x, dZ, out=self.W.grad, transA=True, precision=prec)    # dW = H^T . dZ
+            if _checkpointed(x):
+                K.mx8_weight_grad(x, dZ, out=self.W.grad, precision=prec)
+            else:
+                K.gemm(x, dZ, out=self.W.grad, transA=True, precision=prec)    # dW = H^T . dZ
             after_dw = kwargs.get('after_dw')
             if after_dw is not None:
                 after_dw()            # (partitioned sweep: the sibling convolution's SpMM + return exchange start here)
@@ -579,6 +602,56 @@ class DenseLayer(Layer):
             return [K.gemm(dZ, self.W.data, transB=True, precision=prec)]  # dH = dZ . W^T
         K.spmm_t(x, dZ, out=self.W.grad, precision=kwargs.get('gemm_precision'))      # dW0 = X^T . dS0
         return [None]
+
+
+class GatedDenseLayer(Layer):
+    """y = nonlinearity(x . Wg + bg) * (x . Wu + bu): a dense layer whose units each carry a gate of their own (ops.gated_dense; no
+    reference counterpart, a sibling of the highway block).  ``nonlinearity``: linear, tanh, sigmoid, rectify, swish or gelu.
+    ``checkpoint='mx8'``: the tape keeps x and the two pre-activations in 8 bits instead of fp32 (3.1 bytes for 12) and the backward runs
+    from the codes."""
+
+    def __init__(self, incoming, num_units, Wg=_init.GlorotUniform(), Wu=_init.GlorotUniform(), bg=_init.Constant(0.), bu=_init.Constant(0.),
+                 nonlinearity=_nl.sigmoid, name=None, checkpoint=None):
+        super().__init__(incoming, name)
+        self.nonlinearity = _nl.resolve(nonlinearity)
+        if self.nonlinearity.gate is None:
+            raise ValueError("nonlinearity %s cannot gate" % self.nonlinearity.name)
+        if (bg is None) != (bu is None):
+            raise ValueError("a gated layer has both biases or none")
+        self.num_units = int(num_units)
+        self.checkpoint = _check_checkpoint(checkpoint)
+        num_inputs = int(np.prod(self.input_shape[1:]))
+        self.Wg = self.add_param(Wg, (num_inputs, self.num_units), name="Wg")
+        self.Wu = self.add_param(Wu, (num_inputs, self.num_units), name="Wu")
+        self.bg = None if bg is None else self.add_param(bg, (self.num_units,), name="bg", regularizable=False)
+        self.bu = None if bu is None else self.add_param(bu, (self.num_units,), name="bu", regularizable=False)
+
+    def get_output_shape_for(self, input_shape):
+        return (input_shape[0], self.num_units)
+
+    def forward(self, input, tape, **kwargs):
+        K = backend.active()
+        if not isinstance(input, K.DMat):
+            raise ValueError("Input for this layer must be dense")
+        if self.Wg.data is None:
+            raise RuntimeError("parameters are not on the device yet: bind them with ParamStore")
+        b = (None, None) if self.bg is None else (self.bg.data, self.bu.data)
+        args = dict(act=self.nonlinearity.gate, precision=kwargs.get('gemm_precision'))
+        if tape is None:
+            return K.gated_dense(input, self.Wg.data, self.Wu.data, *b, **args)
+        y, kept = K.gated_dense(input, self.Wg.data, self.Wu.data, *b, keep=self.checkpoint or 'full', **args)
+        tape[self] = {'x': input if self.checkpoint is None else K.mx8_pack(input), 'kept': kept}
+        return y
+
+    def backward(self, grad, tape, into, need_input_grad=True, **kwargs):
+        K = backend.active()
+        s = tape[self]
+        db = (None, None) if self.bg is None else (self.bg.grad, self.bu.grad)
+        dx = K.gated_dense_bwd(grad, s['x'], self.Wg.data, self.Wu.data, s['kept'], act=self.nonlinearity.gate, dWg=self.Wg.grad, dWu=self.Wu.grad,
+                               dbg=db[0], dbu=db[1], need_input_grad=need_input_grad, precision=kwargs.get('gemm_precision'))[0]
+        if dx is not None and into[0] is not None:
+            return [_accumulate(into[0], dx)]
+        return [dx]
 
 
 class DropoutLayer(Layer):
@@ -794,7 +867,9 @@ def get_output(layer_or_layers, inputs=None, tape=None, **kwargs):
                 started.add(nxt)
         values[layer] = layer.forward(x, tape, **kwargs)
     if tape is not None:
-        tape['__values__'] = values
+        # (what a checkpointing layer reads is on the tape in 8 bits: the tape does not hold it whole as well)
+        packed = {l.input_layer for l in all_layers if getattr(l, 'checkpoint', None) is not None}
+        tape['__values__'] = {l: v for l, v in values.items() if l not in packed} if packed else values
     try:
         return [values[l] for l in layer_or_layers]
     except TypeError:
