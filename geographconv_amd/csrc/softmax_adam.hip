@@ -295,6 +295,12 @@ __global__ void adam_next_step_kernel(int64_t* state, float lr, float b1, float 
     reinterpret_cast<float*>(state + 1)[0] = adam_a_t(lr, b1, b2, (float)t);
 }
 
+// a b + c d with both products rounded on their own, whatever the compiler would fuse: the update's bits do not hang on its choice
+__device__ __forceinline__ float adam_sum(float a, float b, float c, float d) {
+#pragma clang fp contract(off)
+    const float ab = a * b, cd = c * d;
+    return ab + cd;
+}
 __global__ __launch_bounds__(TPB) void adam_kernel(int64_t n, float* __restrict__ p, float* __restrict__ g,
                                                    float* __restrict__ m, float* __restrict__ v,
                                                    const float* __restrict__ regmask, float a_t,
@@ -306,11 +312,11 @@ __global__ __launch_bounds__(TPB) void adam_kernel(int64_t n, float* __restrict_
         float gi = g[i];
         if (regmask) {
             const float sgn = (pi > 0.f) ? 1.f : ((pi < 0.f) ? -1.f : 0.f);
-            gi += regmask[i] * (l1 * sgn + 2.0f * l2 * pi);
+            gi = fmaf(regmask[i], adam_sum(l1, sgn, 2.0f * l2, pi), gi);
             g[i] = gi;              // g now holds d(train_loss)/dp including the penalty
         }
-        const float mi = b1 * m[i] + (1.0f - b1) * gi;
-        const float vi = b2 * v[i] + (1.0f - b2) * gi * gi;
+        const float mi = adam_sum(b1, m[i], 1.0f - b1, gi);
+        const float vi = adam_sum(b2, v[i], (1.0f - b2) * gi, gi);
         m[i] = mi;
         v[i] = vi;
         p[i] = pi - a_t * mi / (sqrtf(vi) + eps);
