@@ -25,19 +25,23 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kOob = 0x80000000u;
 
-// ---- a matrix -> its bf16 term planes -----------------------------------------------------------------------------------------------------
+// ---- matrices -> their bf16 term planes: up to three of one storage type in one launch (grid.y) ----------------------------------------------
+struct TermsJobs {
+    int n;
+    struct Job { MatIn src; int64_t total, ldo, plane; int F, qpr; uint16_t* out; } job[3];
+};
 template <int P, int TYPE>
-__global__ __launch_bounds__(256) void terms_kernel(MatIn src, int64_t n, int F, int qpr, uint16_t* __restrict__ out, int64_t ldo, int64_t plane) {
-    const int64_t total = n * qpr;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-        const int64_t r = q / qpr;
-        const int c = (int)(q - r * qpr) * 4;
+__global__ __launch_bounds__(256) void terms_kernel(const TermsJobs jobs) {
+    const TermsJobs::Job& j = jobs.job[blockIdx.y];
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < j.total; q += (int64_t)gridDim.x * 256) {
+        const int64_t r = q / j.qpr;
+        const int c = (int)(q - r * j.qpr) * 4;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < F) x = mask4(mat_load4<TYPE>(src, r, c), c, F);
+        if (c < j.F) x = mask4(mat_load4<TYPE>(j.src, r, c), c, j.F);
         uint2 t[P];
         bf16_terms4<P>(x, t);
 #pragma unroll
-        for (int p = 0; p < P; ++p) *reinterpret_cast<uint2*>(out + p * plane + r * ldo + c) = t[p];
+        for (int p = 0; p < P; ++p) *reinterpret_cast<uint2*>(j.out + p * j.plane + r * j.ldo + c) = t[p];
     }
 }
 
@@ -768,21 +772,23 @@ struct Arena {
 // an operand as the tiled kernel reads it
 struct Planes { const uint16_t* p; int64_t ld, plane; };
 
-// in place where a bf16 matrix's rows start on 16 bytes (and its k-extent is whole pieces, `whole_cols`), else term planes in the workspace
-int make_planes(Arena& ar, const MatIn& m, int64_t n, int64_t F, int P, bool whole_cols, hipStream_t st, Planes* out) {
-    if (m.type == GEOGCN_T_BF16 && m.ld % 8 == 0 && aligned16(m.p) && (!whole_cols || F % 8 == 0)) {
-        *out = Planes{static_cast<const uint16_t*>(m.p), m.ld, 0};
-        return 0;
-    }
+// in place where a bf16 matrix's rows start on 16 bytes (and its k-extent is whole pieces, `whole_cols`), else term planes in the workspace,
+// written by the launch that run_terms makes of all jobs gathered in `jobs`
+Planes make_planes(Arena& ar, const MatIn& m, int64_t n, int64_t F, int P, bool whole_cols, TermsJobs& jobs) {
+    if (m.type == GEOGCN_T_BF16 && m.ld % 8 == 0 && aligned16(m.p) && (!whole_cols || F % 8 == 0)) return Planes{static_cast<const uint16_t*>(m.p), m.ld, 0};
     const int64_t plane = up(F, 64), ld = P * plane;
     uint16_t* o = static_cast<uint16_t*>(ar.take(n * ld * 2));
-    *out = Planes{o, ld, plane};
-    if (ar.counting || n * ld == 0) return 0;
-    const int qpr = (int)(plane / 4);
-    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(n * qpr, 256), (int64_t)kNumCU * 32);
-    auto* k = P == 3 ? &terms_kernel<3, GEOGCN_T_F32> : m.type == GEOGCN_T_F32 ? &terms_kernel<1, GEOGCN_T_F32>
-              : m.type == GEOGCN_T_BF16 ? &terms_kernel<1, GEOGCN_T_BF16> : &terms_kernel<1, GEOGCN_T_MX8>;          // (three terms: fp32 only)
-    hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, st, m, n, (int)F, qpr, o, ld, plane);
+    if (n * ld > 0) jobs.job[jobs.n++] = TermsJobs::Job{m, n * (plane / 4), ld, plane, (int)F, (int)(plane / 4), o};
+    return Planes{o, ld, plane};
+}
+int run_terms(const Arena& ar, const TermsJobs& jobs, int P, hipStream_t st) {
+    if (ar.counting || jobs.n == 0) return 0;
+    const int type = jobs.job[0].src.type;
+    int64_t most = 0;
+    for (int i = 0; i < jobs.n; ++i) most = std::max(most, jobs.job[i].total);
+    auto* k = P == 3 ? &terms_kernel<3, GEOGCN_T_F32> : type == GEOGCN_T_F32 ? &terms_kernel<1, GEOGCN_T_F32>
+              : type == GEOGCN_T_BF16 ? &terms_kernel<1, GEOGCN_T_BF16> : &terms_kernel<1, GEOGCN_T_MX8>;          // (three terms: fp32 only)
+    hipLaunchKernelGGL(k, dim3((unsigned)std::min<int64_t>(cdiv(most, 256), (int64_t)kNumCU * 32), jobs.n), dim3(256), 0, st, jobs);
     GEOGCN_LAUNCH_CHECK("terms_kernel");
     return 0;
 }
@@ -832,11 +838,13 @@ int run_tiles(Arena& ar, TileArgs& t, const Cut& c, hipStream_t st) {
     return finish(t, NSEG, GATED ? EPI_GATED : EPI_STORE, st);
 }
 
-// Which tile shape, and how many ways the reduction is split: the pair with the least estimated time, in clocks -- the busiest CU's share of
-// the products at half of the matrix pipe's rate times the shape's measured standing (`eff`: 1 for the fastest of its list on a large product),
-// plus, for a split, its slabs written and read back at the rate of a large copy and one more launch.
+// Which tile shape, and how many ways the reduction is split: the pair with the least estimated time, in clocks.  The busiest CU has R tiles, `per_cu`
+// of them at a time: it takes the products of R tiles at 0.7 of the matrix pipe's rate times the shape's measured standing (`eff`: 1 for the
+// fastest of its list on a large product), or, where few blocks are there to cover for each other, a load's latency (1,900) for every
+// stage that is not asked for ahead; a tile begins and ends in 6,000.  A split writes and reads its slabs (1,500 bytes a clock) and
+// takes one more launch.
 struct Shape {
-    int bm, bns, bk;
+    int bm, bns, bk, stages, per_cu;
     double eff;
     int (*run)(Arena&, TileArgs&, const Cut&, hipStream_t);
 };
@@ -849,9 +857,10 @@ int run_best(const Shape (&shapes)[N], Arena& ar, TileArgs& t, int64_t cols, int
         const int64_t n_mt = cdiv(t.M, s.bm), n_nt = cdiv(cols, s.bns), tiles = n_mt * n_nt;
         const int64_t steps = std::max<int64_t>(1, t.n_kseg * cdiv(t.K[0], s.bk));
         for (int64_t want = 1; want == 1 || (want <= steps / 4 && tiles * want <= 2 * kNumCU); want += want < 8 ? 1 : want / 4) {
-            const int64_t per = cdiv(steps, want), nsplit = cdiv(steps, per);
-            double clk = (double)cdiv(tiles * nsplit, kNumCU) * s.bm * s.bns * nseg * (per * s.bk) * terms / (2048 * 0.5 * s.eff);
-            if (nsplit > 1) clk += 2.0 * nsplit * t.M * n_nt * s.bns * nseg * 4 / 2200 + 8000;
+            const int64_t per = cdiv(steps, want), nsplit = cdiv(steps, per), R = cdiv(tiles * nsplit, kNumCU), turns = cdiv(R, s.per_cu);
+            const double products = (double)R * s.bm * s.bns * nseg * (per * s.bk) * terms / (2048 * 0.7 * s.eff);
+            double clk = std::max(products, (double)turns * per * 1900 / (s.stages - 1)) + turns * 6000.0;
+            if (nsplit > 1) clk += 2.0 * nsplit * t.M * n_nt * s.bns * nseg * 4 / 1500 + 16000;
             if (!pick || clk < best) {
                 best = clk;
                 pick = &s;
@@ -865,37 +874,42 @@ int run_best(const Shape (&shapes)[N], Arena& ar, TileArgs& t, int64_t cols, int
 // X.[Wg | Wu] and the gate.  (Shapes of two blocks a CU where LDS and registers allow: one block's epilogue and barriers run under the other's
 // products.  8192 x 2048 -> 8192 in bf16: 128 x 256 531-660 us by box, the same with 64 k-values a stage and one block a CU 650-790.)
 int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
-    static const Shape fp32[] = {{128, 128, 32, 1.0, run_tiles<3, 3, false, true, 2, 128, 256, 32, 2, 4, 2, true>},
-                                 {256, 64, 32, 0.95, run_tiles<3, 3, false, true, 2, 256, 128, 32, 4, 2, 2, true>},
-                                 {64, 64, 32, 0.85, run_tiles<3, 3, false, true, 2, 64, 128, 32, 2, 2, 2, true>}};
-    static const Shape bf16[] = {{128, 128, 32, 1.0, run_tiles<1, 1, false, true, 2, 128, 256, 32, 2, 4, 3, true>},
-                                 {256, 64, 32, 0.97, run_tiles<1, 1, false, true, 2, 256, 128, 32, 4, 2, 3, true>},
-                                 {128, 64, 32, 0.88, run_tiles<1, 1, false, true, 2, 128, 128, 32, 4, 2, 3, true>}};
+    static const Shape fp32[] = {{128, 128, 32, 2, 1, 1.0, run_tiles<3, 3, false, true, 2, 128, 256, 32, 2, 4, 2, true>},
+                                 {256, 64, 32, 2, 1, 0.95, run_tiles<3, 3, false, true, 2, 256, 128, 32, 4, 2, 2, true>},
+                                 {64, 64, 32, 2, 2, 0.85, run_tiles<3, 3, false, true, 2, 64, 128, 32, 2, 2, 2, true>}};
+    static const Shape bf16[] = {{128, 128, 32, 3, 2, 1.0, run_tiles<1, 1, false, true, 2, 128, 256, 32, 2, 4, 3, true>},
+                                 {256, 64, 32, 3, 2, 0.97, run_tiles<1, 1, false, true, 2, 256, 128, 32, 4, 2, 3, true>},
+                                 {128, 64, 32, 3, 3, 0.88, run_tiles<1, 1, false, true, 2, 128, 128, 32, 4, 2, 3, true>},
+                                 {128, 64, 32, 5, 2, 0.87, run_tiles<1, 1, false, true, 2, 128, 128, 32, 4, 2, 5, true>},
+                                 {128, 64, 64, 4, 1, 0.8, run_tiles<1, 1, false, true, 2, 128, 128, 64, 4, 2, 4, true>}};
     const int64_t cols = t.keep == GEOGCN_KEEP_MX8 ? std::max(t.ncols, up(t.N, kMxBlock)) : t.ncols;
     return P == 3 ? run_best(fp32, ar, t, cols, 2, 6, st) : run_best(bf16, ar, t, cols, 2, 1, st);
 }
 
 // dG.Wg^T + dU.Wu^T: both operands run along k, so the one-term shapes take 64 k-values a stage (whole 128-byte lines of a row)
 int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
-    static const Shape fp32[] = {{256, 160, 32, 1.0, run_tiles<3, 3, false, false, 1, 256, 160, 32, 4, 2, 2, false>},
-                                 {256, 128, 32, 0.92, run_tiles<3, 3, false, false, 1, 256, 128, 32, 4, 2, 2, false>},
-                                 {64, 128, 32, 0.68, run_tiles<3, 3, false, false, 1, 64, 128, 32, 2, 2, 2, false>}};
-    static const Shape bf16[] = {{256, 256, 64, 1.0, run_tiles<1, 1, false, false, 1, 256, 256, 64, 2, 4, 2, false>},
-                                 {256, 128, 64, 0.85, run_tiles<1, 1, false, false, 1, 256, 128, 64, 4, 2, 3, false>},
-                                 {128, 128, 64, 0.8, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 2, false>}};
+    static const Shape fp32[] = {{256, 160, 32, 2, 1, 1.0, run_tiles<3, 3, false, false, 1, 256, 160, 32, 4, 2, 2, false>},
+                                 {256, 128, 32, 2, 1, 0.92, run_tiles<3, 3, false, false, 1, 256, 128, 32, 4, 2, 2, false>},
+                                 {64, 128, 32, 2, 2, 0.68, run_tiles<3, 3, false, false, 1, 64, 128, 32, 2, 2, 2, false>}};
+    static const Shape bf16[] = {{256, 256, 64, 2, 1, 1.0, run_tiles<1, 1, false, false, 1, 256, 256, 64, 2, 4, 2, false>},
+                                 {256, 128, 64, 3, 1, 0.85, run_tiles<1, 1, false, false, 1, 256, 128, 64, 4, 2, 3, false>},
+                                 {128, 128, 64, 2, 2, 0.8, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 2, false>},
+                                 {128, 128, 64, 4, 1, 0.75, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 4, false>}};
     return P == 3 ? run_best(fp32, ar, t, t.ncols, 1, 6, st) : run_best(bf16, ar, t, t.ncols, 1, 1, st);
 }
 
 // X^T.[B0 | B1] (nseg = 2) or X^T.B0
 int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_t st) {
-    static const Shape fp32[] = {{128, 128, 32, 1.0, run_tiles<3, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
-    static const Shape mx8[] = {{160, 160, 32, 1.0, run_tiles<1, 3, true, true, 2, 160, 320, 32, 2, 4, 2, false>},
-                                {128, 128, 32, 0.85, run_tiles<1, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
-    static const Shape bf16[] = {{128, 128, 64, 1.0, run_tiles<1, 1, true, true, 2, 128, 256, 64, 2, 4, 2, false>},
-                                 {128, 64, 64, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 2, 2, false>}};
-    static const Shape mx8_one[] = {{160, 256, 32, 1.0, run_tiles<1, 3, true, true, 1, 160, 256, 32, 2, 4, 2, false>},
-                                    {128, 128, 32, 0.8, run_tiles<1, 3, true, true, 1, 128, 128, 32, 2, 4, 5, false>}};
-    static const Shape bf16_one[] = {{128, 128, 32, 1.0, run_tiles<1, 1, true, true, 1, 128, 128, 32, 2, 4, 6, false>}};
+    static const Shape fp32[] = {{128, 128, 32, 2, 1, 1.0, run_tiles<3, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
+    static const Shape mx8[] = {{160, 160, 32, 2, 1, 1.0, run_tiles<1, 3, true, true, 2, 160, 320, 32, 2, 4, 2, false>},
+                                {128, 128, 32, 2, 1, 0.85, run_tiles<1, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
+    static const Shape bf16[] = {{128, 128, 64, 3, 1, 1.0, run_tiles<1, 1, true, true, 2, 128, 256, 64, 2, 4, 3, false>},
+                                 {128, 64, 64, 2, 2, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 2, 2, false>},
+                                 {128, 64, 64, 4, 1, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 4, 4, false>},
+                                 {128, 64, 32, 5, 2, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 32, 2, 4, 5, false>}};
+    static const Shape mx8_one[] = {{160, 256, 32, 2, 1, 1.0, run_tiles<1, 3, true, true, 1, 160, 256, 32, 2, 4, 2, false>},
+                                    {128, 128, 32, 5, 1, 0.8, run_tiles<1, 3, true, true, 1, 128, 128, 32, 2, 4, 5, false>}};
+    static const Shape bf16_one[] = {{128, 128, 32, 6, 1, 1.0, run_tiles<1, 1, true, true, 1, 128, 128, 32, 2, 4, 6, false>}};
     if (nseg == 2) {
         if (PA == 3) return run_best(fp32, ar, t, t.ncols, 2, 6, st);
         return PB == 3 ? run_best(mx8, ar, t, t.ncols, 2, 3, st) : run_best(bf16, ar, t, t.ncols, 2, 1, st);
@@ -1019,10 +1033,10 @@ int forward(Arena& ar, const FwdArgs& f, hipStream_t st) {
         return ar.counting ? 0 : x3_run_rows(kc, false, call, w, st);
     }
     const int P = terms_of(f.type, f.precision);
-    Planes x, wg, wu;
-    if (const int rc = make_planes(ar, f.X, f.M, f.K, P, true, st, &x)) return rc;
-    if (const int rc = make_planes(ar, f.Wg, f.K, f.N, P, false, st, &wg)) return rc;
-    if (const int rc = make_planes(ar, f.Wu, f.K, f.N, P, false, st, &wu)) return rc;
+    TermsJobs jobs{};
+    const Planes x = make_planes(ar, f.X, f.M, f.K, P, true, jobs), wg = make_planes(ar, f.Wg, f.K, f.N, P, false, jobs),
+                 wu = make_planes(ar, f.Wu, f.K, f.N, P, false, jobs);
+    if (const int rc = run_terms(ar, jobs, P, st)) return rc;
     TileArgs t = tile_args();
     t.M = f.M; t.N = f.N; t.K[0] = f.K;
     t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
@@ -1146,10 +1160,21 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
     const int64_t plane = up(b.N, 64), ldo = P * plane;
     uint16_t *dG, *dU;
     if (const int rc = gate_gradients(ar, b, P, plane, st, &dG, &dU)) return rc;
+    TermsJobs jobs{};
+    Planes wg{}, wu{}, x{};
     if (b.dX) {
-        Planes wg, wu;
-        if (const int rc = make_planes(ar, b.Wg, b.K, b.N, P, true, st, &wg)) return rc;
-        if (const int rc = make_planes(ar, b.Wu, b.K, b.N, P, true, st, &wu)) return rc;
+        wg = make_planes(ar, b.Wg, b.K, b.N, P, true, jobs);
+        wu = make_planes(ar, b.Wu, b.K, b.N, P, true, jobs);
+    }
+    if (b.dW[0] && b.X.type != b.Wg.type) {                   // (a checkpointed X: a storage type of its own)
+        TermsJobs own{};
+        x = make_planes(ar, b.X, b.M, b.K, PX, false, own);
+        if (const int rc = run_terms(ar, own, PX, st)) return rc;
+    } else if (b.dW[0]) {
+        x = make_planes(ar, b.X, b.M, b.K, PX, false, jobs);
+    }
+    if (const int rc = run_terms(ar, jobs, P, st)) return rc;
+    if (b.dX) {
         TileArgs t = tile_args();
         t.M = b.M; t.N = b.K; t.n_kseg = 2; t.K[0] = t.K[1] = b.N;
         t.A[0] = dG; t.A[1] = dU;
@@ -1160,8 +1185,6 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
         if (const int rc = run_input_grad(ar, t, P, st)) return rc;
     }
     if (b.dW[0]) {
-        Planes x;
-        if (const int rc = make_planes(ar, b.X, b.M, b.K, PX, false, st, &x)) return rc;
         TileArgs t = tile_args();
         t.M = b.K; t.N = b.N; t.K[0] = b.M;
         t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
@@ -1193,9 +1216,10 @@ int weight_grad(Arena& ar, const WgradArgs& w, hipStream_t st) {
         return tn_q8(ar, w.X, w.M, w.K, w.N, 1, B, w.dZ.ld, &w.dW, &w.lddw, st);
     }
     const int P = terms_of(w.type, w.precision);
-    Planes x, dz;
-    if (const int rc = make_planes(ar, w.X, w.M, w.K, 1, false, st, &x)) return rc;
-    if (const int rc = make_planes(ar, w.dZ, w.M, w.N, P, false, st, &dz)) return rc;
+    TermsJobs jx{}, jz{};
+    const Planes x = make_planes(ar, w.X, w.M, w.K, 1, false, jx), dz = make_planes(ar, w.dZ, w.M, w.N, P, false, jz);
+    if (const int rc = run_terms(ar, jx, 1, st)) return rc;
+    if (const int rc = run_terms(ar, jz, P, st)) return rc;
     TileArgs t = tile_args();
     t.M = w.K; t.N = w.N; t.K[0] = w.M;
     t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
