@@ -929,6 +929,8 @@ int elem_align(int type) { return type == GEOGCN_T_F32 ? 16 : type == GEOGCN_T_B
 int check_mat(const char* who, const char* name, int type, const void* p, int64_t ld, const uint8_t* scale, int64_t F) {
     GEOGCN_REQUIRE(p, GEOGCN_E_NULL, "%s: %s is null", who, name);
     GEOGCN_REQUIRE(reinterpret_cast<uintptr_t>(p) % elem_align(type) == 0, GEOGCN_E_ALIGN, "%s: %s is not aligned", who, name);
+    // (a tile's 256 rows are addressed with 32 bits)
+    GEOGCN_REQUIRE(ld <= (1 << 21), GEOGCN_E_SIZE, "%s: pitch %lld of %s is too large", who, (long long)ld, name);
     if (type == GEOGCN_T_MX8) {
         GEOGCN_REQUIRE(scale, GEOGCN_E_NULL, "%s: %s has no scales", who, name);
         GEOGCN_REQUIRE(ld % kMxBlock == 0 && ld >= F, GEOGCN_E_ALIGN, "%s: code pitch %lld of %s (%lld columns) is not whole blocks", who,

@@ -1188,9 +1188,12 @@ class MX8Mat:
 
     @staticmethod
     def empty(n, F, device, bf16=False):
-        w = (int(F) + 31) // 32
-        return MX8Mat(n, F, torch.empty((int(n), 32 * w), dtype=torch.uint8, device=device),
-                      torch.empty((int(n), w), dtype=torch.uint8, device=device), bf16)
+        m = MX8Mat.__new__(MX8Mat)
+        m.n, m.F, m.bf16 = int(n), int(F), bool(bf16)
+        w = (m.F + 31) // 32
+        m.codes = torch.empty((m.n, 32 * w), dtype=torch.uint8, device=device)
+        m.scales = torch.empty((m.n, w), dtype=torch.uint8, device=device)
+        return m
 
     @property
     def ld(self):
@@ -1238,24 +1241,39 @@ def _ptr(t):
 
 
 def _new_like_block(bf16, n, F, device, ld=None):
-    """Uninitialised: the kernels here write the pad columns themselves."""
-    if bf16:
-        return HMat(n, F, device, ld=ld)
-    return DMat(n, F, t=torch.empty((n, ld or pad4(F)), dtype=torch.float32, device=device))
+    """Uninitialised: the kernels here write the pad columns themselves.  (Built without the constructor's checks of a foreign tensor: a call
+    on a few rows takes 10 us in all.)"""
+    m = HMat.__new__(HMat) if bf16 else DMat.__new__(DMat)
+    m.n, m.F = n, F
+    m.t = torch.empty((n, ld or (bf16_ld(F) if bf16 else pad4(F))), dtype=torch.bfloat16 if bf16 else torch.float32, device=device)
+    return m
 
 
 def _tensor(m):
     return m if m is None or isinstance(m, torch.Tensor) else m.codes if isinstance(m, MX8Mat) else m.t
 
 
-def _same_device(*ms):
+def _same_device(first, *rest):
     """-> the index of the one GPU that all operands (None: absent) live on"""
-    at = [t.get_device() for t in map(_tensor, ms) if t is not None]
-    if min(at) != max(at):
-        raise ValueError("operands live on different devices: %s" % sorted({str(_tensor(m).device) for m in ms if m is not None}))
-    if at[0] < 0:
+    at = _tensor(first).get_device()
+    for m in rest:
+        if m is not None and (m.t if type(m) is DMat or type(m) is HMat else _tensor(m)).get_device() != at:
+            raise ValueError("operands live on different devices: %s" % sorted({str(_tensor(o).device) for o in (first, *rest) if o is not None}))
+    if at < 0:
         raise _ffi.GeoGcnError("operands live in host memory: there is no CPU path")
-    return at[0]
+    return at
+
+
+def _check_apart(who, outs, ins):
+    """Given outputs overlap neither each other nor an operand (they are written while operands are still read)."""
+    def span(m):
+        t = _tensor(m)
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+    spans = [(o, *span(o)) for o in outs if o is not None]
+    for i, (o, a, b) in enumerate(spans):
+        for _, c, d in [(None, *span(m)) for m in ins if m is not None] + spans[:i]:
+            if a < d and c < b:
+                raise ValueError("%s: an output overlaps another operand" % who)
 
 
 def _check_out(m, n, F, kind, what):
@@ -1270,18 +1288,18 @@ def _check_vec(v, N, what):
     return v
 
 
-def _call(fn, name, *args):
-    """One C entry point on the current stream of the current device."""
-    check(fn(*args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())), name)
+def _call(fn, name, index, *args):
+    """One C entry point on the current stream of device `index` (the current one)."""
+    check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), name)
 
 
-def _call_with_ws(fn, name, *args):
+def _call_with_ws(fn, name, index, *args):
     """... of one that says what scratch it needs (GEOGCN_E_WORKSPACE): allocated for this call alone -- stream-ordered, and a captured call's
     lives in the graph's pool, so two graphs never share one."""
-    need, st = C.c_size_t(0), torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    need, st = C.c_size_t(0), torch._C._cuda_getCurrentRawStream(index)
     rc = fn(*args, None, need, st)
     if rc == _ffi.E_WORKSPACE:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=torch.cuda.current_device())
+        ws = torch.empty(need.value, dtype=torch.uint8, device=torch.device('cuda', index))
         rc = fn(*args, ws.data_ptr(), need, st)
     check(rc, name)
 
@@ -1289,10 +1307,10 @@ def _call_with_ws(fn, name, *args):
 def _on_device(index, call, fn, name, *args):
     """`call` (_call / _call_with_ws) with the operands' device current."""
     if torch.cuda.current_device() == index:
-        call(fn, name, *args)
+        call(fn, name, index, *args)
     else:
         with torch.cuda.device(index):
-            call(fn, name, *args)
+            call(fn, name, index, *args)
 
 
 @_timed('mx8_pack')
@@ -1373,7 +1391,7 @@ def gated_dense(X, Wg, Wu, bg: torch.Tensor = None, bu: torch.Tensor = None, act
     """act(X . Wg + bg) * (X . Wu + bu), both projections, the activation and the product in one kernel.  All matrices DMat, or all
     HMat (bf16 storage, fp32 accumulation; biases stay fp32).  `keep`: None -> the result alone; 'full' / 'mx8' -> (result, GatedTape) with
     G and U kept in the block's type / in 8 bits for gated_dense_bwd.  `precision` (fp32 block): 'bf16x3', 'bf16', or 'f32' -- the exact
-    fp32 products, in their own launches."""
+    fp32 products, in their own launches.  Up to 16 rows are multiplied in plain fp32 ('bf16x3' and 'f32').  `out` overlaps no operand."""
     if keep not in (None, 'full', 'mx8'):
         raise ValueError("gated_dense: keep is None, 'full' or 'mx8', not %r" % (keep,))
     if isinstance(X, MX8Mat):
@@ -1385,6 +1403,8 @@ def gated_dense(X, Wg, Wu, bg: torch.Tensor = None, bu: torch.Tensor = None, act
     kind = HMat if bf16 else DMat
     H = _new_like_block(bf16, M, N, X.device) if out is None else _check_out(out, M, N, kind, 'gated_dense: the output')
     index = _same_device(X, Wg, Wu, bg, bu, H)
+    if out is not None:
+        _check_apart('gated_dense', [out], [X, Wg, Wu, bg, bu])
     G = U = None
     if keep == 'full':
         G, U = (_new_like_block(bf16, M, N, X.device, H.ld) for _ in range(2))
@@ -1416,6 +1436,8 @@ def gated_dense_bwd(dH, X, Wg, Wu, kept: GatedTape, act=ACT_SIGMOID, dX=None, dW
             _check_out(m, n, F, kind, 'gated_dense_bwd: ' + what)
     prec = _block_precision(precision, bf16)
     index, dev = _same_device(dH, X, Wg, Wu, kept.G, kept.U, dX, dWg, dWu, dbg, dbu), dH.device
+    if dX is not None or dWg is not None or dbg is not None:
+        _check_apart('gated_dense_bwd', [dX, dWg, dWu, dbg, dbu], [dH, X, Wg, Wu, kept.G, kept.U])
     bias = bias or dbg is not None
     if bias and dbg is None:
         dbg, dbu = ((torch.zeros if N % 4 else torch.empty)(pad4(N), dtype=torch.float32, device=dev) for _ in range(2))

@@ -512,6 +512,7 @@ int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, 
  * gives NaN.)  Products of bf16 matrices are one kind, whatever `precision` says.
  * keep: what of G = X.Wg + bg and U = X.Wu + bu is stored for the backward -- nothing, in the block's type (pitch >= H's), or as 8-bit
  * checkpoints (codes G / U with pitch ldg / ldu and scales Gs / Us as geogcn_mx8_pack writes them).
+ * K, N <= 2^20, pitches <= 2^21.  H, G, U, dX, dWg, dWu overlap none of the other matrices.
  * ws: scratch of *ws_bytes bytes, 256-byte aligned (may be NULL).  A call that needs more launches nothing, sets *ws_bytes to what it needs and
  * returns GEOGCN_E_WORKSPACE; calls of a few rows need none.  How operands are read depends on their addresses: ask with the very
  * arguments of the call.  Nothing in ws outlives the call.                                                                               */

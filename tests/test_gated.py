@@ -87,6 +87,17 @@ def test_wrong_arguments_are_refused(call):
         call()
 
 
+def test_overlapping_outputs_are_refused():
+    x, w = D(8, 8), D(8, 8)
+    with pytest.raises(ValueError):
+        ops._check_apart('x', [x], [w, x])
+    big = D(20, 8)
+    for outs, ins in (([big.rows(0, 8)], [big.rows(7, 15)]), ([x, x], [w]), ([big.rows(2, 4), big.rows(3, 5)], [])):
+        with pytest.raises(ValueError):
+            ops._check_apart('x', outs, ins)
+    ops._check_apart('x', [big.rows(0, 8), None], [big.rows(8, 16), None, x])
+
+
 @pytest.mark.parametrize('call', [
     lambda: ops.gated_dense(D(4, 8), D(8, 12), D(8, 12)),
     lambda: ops.gated_dense_bwd(D(4, 12), D(4, 8), D(8, 12), D(8, 12), ops.GatedTape(D(4, 12), D(4, 12))),
@@ -114,7 +125,7 @@ def test_c_entry_refusals(lib):
     assert _fwd(lib)[0] == _ffi.E_WORKSPACE and _fwd(lib)[1] > 0
     for kw, rc in ((dict(M=-1), -2), (dict(N=1 << 21), -2), (dict(type=2), -4), (dict(act=3), -4), (dict(act=7), -4), (dict(keep=3), -4),
                    (dict(precision=3), -4), (dict(X=None), -1), (dict(Wu=None), -1), (dict(H=None), -1), (dict(X=4100), -3), (dict(ldx=18), -3),
-                   (dict(ldx=12), -3), (dict(ldh=28), -3), (dict(H=16392), -3), (dict(keep=1), -1), (dict(keep=2, G=64, ldg=32, U=64, ldu=32), -1),
+                   (dict(ldx=12), -3), (dict(ldx=1 << 22), -2), (dict(ldh=28), -3), (dict(H=16392), -3), (dict(keep=1), -1), (dict(keep=2, G=64, ldg=32, U=64, ldu=32), -1),
                    (dict(keep=2, G=64, ldg=48, Gs=64, U=64, ldu=32, Us=64), -3), (dict(keep=1, type=1, ldh=64, G=64, ldg=32, U=64, ldu=64), -3)):
         got = _fwd(lib, **kw)[0]
         assert got == rc, (kw, got)

@@ -232,6 +232,18 @@ def test_pitches_junk_pads_and_neighbouring_rows(dev, dtype):
            _forward_bounds(dict(r, bg=np.zeros(N)), 'silu', dtype)[0], 'one bias')
 
 
+def test_outputs_that_overlap_operands_are_refused(dev):
+    from geographconv_amd import ops
+    d, _ = _problem(dev, 20, 32, 32, 'f32', True, 1)
+    _, kept = ops.gated_dense(d['X'], d['Wg'], d['Wu'], keep='full')
+    dH = _mat(_rand((20, 32), 2), dev, 'f32')
+    for call in (lambda: ops.gated_dense(d['X'], d['Wg'], d['Wu'], out=d['X']),
+                 lambda: ops.gated_dense_bwd(dH, d['X'], d['Wg'], d['Wu'], kept, dX=d['X']),
+                 lambda: ops.gated_dense_bwd(dH, d['X'], d['Wg'], d['Wu'], kept, dWg=d['Wg'], dWu=_mat(_rand((32, 32), 3), dev, 'f32'))):
+        with pytest.raises(ValueError):
+            call()
+
+
 @pytest.mark.parametrize('dtype', ['f32', 'bf16'])
 def test_empty_sizes(dev, dtype):
     from geographconv_amd import ops
