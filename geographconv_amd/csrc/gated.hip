@@ -880,7 +880,6 @@ int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
     static const Shape bf16[] = {{128, 128, 32, 3, 2, 1.0, run_tiles<1, 1, false, true, 2, 128, 256, 32, 2, 4, 3, true>},
                                  {256, 64, 32, 3, 2, 0.97, run_tiles<1, 1, false, true, 2, 256, 128, 32, 4, 2, 3, true>},
                                  {128, 64, 32, 3, 3, 0.88, run_tiles<1, 1, false, true, 2, 128, 128, 32, 4, 2, 3, true>},
-                                 {128, 64, 32, 5, 2, 0.87, run_tiles<1, 1, false, true, 2, 128, 128, 32, 4, 2, 5, true>},
                                  {128, 64, 64, 4, 1, 0.8, run_tiles<1, 1, false, true, 2, 128, 128, 64, 4, 2, 4, true>}};
     const int64_t cols = t.keep == GEOGCN_KEEP_MX8 ? std::max(t.ncols, up(t.N, kMxBlock)) : t.ncols;
     return P == 3 ? run_best(fp32, ar, t, cols, 2, 6, st) : run_best(bf16, ar, t, cols, 2, 1, st);
@@ -905,8 +904,7 @@ int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_
                                 {128, 128, 32, 2, 1, 0.85, run_tiles<1, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
     static const Shape bf16[] = {{128, 128, 64, 3, 1, 1.0, run_tiles<1, 1, true, true, 2, 128, 256, 64, 2, 4, 3, false>},
                                  {128, 64, 64, 2, 2, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 2, 2, false>},
-                                 {128, 64, 64, 4, 1, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 4, 4, false>},
-                                 {128, 64, 32, 5, 2, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 32, 2, 4, 5, false>}};
+                                 {128, 64, 64, 4, 1, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 4, 4, false>}};
     static const Shape mx8_one[] = {{160, 256, 32, 2, 1, 1.0, run_tiles<1, 3, true, true, 1, 160, 256, 32, 2, 4, 2, false>},
                                     {128, 128, 32, 5, 1, 0.8, run_tiles<1, 3, true, true, 1, 128, 128, 32, 2, 4, 5, false>}};
     static const Shape bf16_one[] = {{128, 128, 32, 6, 1, 1.0, run_tiles<1, 1, true, true, 1, 128, 128, 32, 2, 4, 6, false>}};
