@@ -1063,12 +1063,12 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
     const int64_t ldt = P ? P * ldo : ldo, plane = ldo, bytes = b.M * ldt * (P ? 2 : 4);
     uint16_t* dG = *dG_out = static_cast<uint16_t*>(ar.take(bytes));
     uint16_t* dU = *dU_out = static_cast<uint16_t*>(ar.take(bytes));
-    // quads of columns of a block: all of them, or equal shares where there are more than 256; rows: enough blocks to keep every CU at eight, and
-    // 1,024 rows where they are long anyway
+    // quads of columns of a block: all of them, or equal shares where there are more than 256; rows: enough blocks to keep every CU at eight, not
+    // fewer than eight rows (each block writes a row of partial sums) and 1,024 where they are long anyway
     const int64_t quads = cdiv(ldo, 4), cblocks = cdiv(quads, 256);
     const int qw = (int)cdiv(quads, cblocks), rw = 256 / qw;
-    const int rows = (int)std::max(std::min<int64_t>(1024, std::max<int64_t>(2 * rw, up(cdiv(b.M * cblocks, (int64_t)kNumCU * 8), 2 * rw))),
-                                   up(cdiv(b.M, 65535), 2 * rw));     // (grid.y)
+    const int64_t fill = std::max<int64_t>(8, cdiv(b.M * cblocks, (int64_t)kNumCU * 8));
+    const int rows = (int)up(std::max(std::min<int64_t>(1024, fill), cdiv(b.M, 65535)), 2 * rw);      // (65,535: grid.y)
     const int64_t nparts = cdiv(b.M, rows), part_ld = up(b.N, 4);
     float* part = b.db[0] ? static_cast<float*>(ar.take(2 * nparts * part_ld * 4)) : nullptr;
     if (!ar.counting) {
