@@ -52,6 +52,9 @@ __global__ __launch_bounds__(256) void terms_kernel(const TermsJobs jobs) {
 // read as 16-byte fragments, a k-strided one through the transposing LDS read (4 k-values of a lane's own column).  Both images are
 // permuted in 16-byte pieces so that the lanes of a read phase meet different banks.
 // NSEG = 2: the block's columns are BN / 2 of B[0] and the same BN / 2 of B[1] -- a lane then owns g and u of one element.
+// What bounds it: in bf16 the LDS (a wave's 64 x 64 products of a k-step take 256 clocks of its SIMD and 8 KB of reads; two blocks a CU cover each
+// other's barriers) -- 1.17 PFLOP/s at 16,384 x 4,096 -> 4,096, 1.05 at 8,192 x 2,048 -> 8,192, matrix pipe busy 38-56 %, no bank conflicts; at three
+// terms the clock under power (the products of 60,000 x 600 -> 600: 1.0 PFLOP/s) or, with few tiles, a load's latency per stage.
 struct TileArgs {
     int64_t M, N;                                     // rows of C, columns of each segment of C
     int n_mt, n_nt, nsplit, steps_per_split;
@@ -457,7 +460,8 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
 // A block takes 32 columns of both weights over the whole reduction; its 512 threads read 16 bytes (VEC values) of each weight a step, CL lanes
 // side by side over the columns, KS k-rows at a time, straight from the matrices (no term planes: products are fp32 fmas of the stored
 // values).  x lies in LDS as [k][row].  The partial sums meet in two rotations within 16 lanes and then in LDS, always in the same order.
-// 32 columns are one checkpoint block of a row.  Bound by the latency of the one pass over the weights: 1 x 1024 -> 4096 in bf16 (16.8 MB).
+// 32 columns are one checkpoint block of a row.  Bound by the latency of one round of loads and the reduction: 1 x 1024 -> 4096 in bf16 (16.8 MB)
+// 6.4-7.1 us = 2.4-2.6 TB/s (8.5 + 4.8 us by tiles and a split).
 struct FewArgs {
     int64_t M, ldx, ldwg, ldwu, ncols;
     int K, N, act, out_type, keep;
@@ -668,6 +672,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
 }
 
 // ---- dG, dU as term planes (P = 0: as fp32 matrices), with the partial column sums of both (bias gradients) ------------------------------
+// One pass over dH, G, U, bound by HBM: 440,000 x 300 in fp32 0.57 ms for 2.64 GB (4.6 TB/s, a large copy's rate), from checkpoints 0.39 ms.
 // A block takes `rows` rows of qw * 4 columns; its partial sums are rows / rw sequential adds per thread, then rw.
 template <int P, int TD, int TK>
 __global__ __launch_bounds__(256) void gate_grad_kernel(MatIn dH, MatIn G, MatIn U, int64_t M, int N, int act, uint16_t* __restrict__ oG,
@@ -1089,7 +1094,6 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
     return 0;
 }
 // X^T.[B0 | B1] of a checkpointed X and fp32 matrices by the library's A^T.B kernel: X's codes and the fp32 values are read as they are
-bool tn_q8_takes(int64_t M, int64_t K, int64_t N) { return M >= kWholeRowsMin && K <= 320 && N <= 1024; }
 int tn_q8(Arena& ar, const MatIn& X, int64_t M, int64_t K, int64_t N, int nseg, const float* const* B, int64_t ldb, void* const* dW, const int64_t* lddw,
           hipStream_t st) {
     const int bn = up(N, 256) <= up(N, 320) ? 256 : 320;
@@ -1151,10 +1155,11 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
 }
 int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
     if (b.precision == GEOGCN_GEMM_F32 && b.type == GEOGCN_T_F32) return backward_exact(ar, b, GEOGCN_GEMM_F32, st);
-    // fp32 over many rows and up to 320 inputs (one tile of the library's A^T.B kernel): dG, dU stay fp32 matrices and the library's split-bf16
-    // kernels multiply them (440,000 x 300 -> 300: 2.17 + 0.92 ms by tiles, against 0.86 + 1.07 ms and a gate pass of 0.55; 60,000 x 600 ->
-    // 600: 1.14 against 1.40)
-    if (b.type == GEOGCN_T_F32 && b.precision == GEOGCN_GEMM_BF16X3 && tn_q8_takes(b.M, b.K, b.N))
+    // fp32 over many rows and 192 to 320 inputs (two whole tiles of the library's A^T.B kernel, a column pass of its whole-rows kernel): dG, dU stay
+    // fp32 matrices and the library's split-bf16 kernels multiply them.  So / by tiles: 440,000 x 300 -> 300 2.5 / 3.1 ms, 100,000 x 300 -> 300
+    // 550 / 715 us, 20,000 x 192 -> 640 224 / 242; outside, 100,000 x 160 -> 300 480 / 511 but 20,000 x 160 -> 640 247 / 214, 60,000 x 600 ->
+    // 600 1.40 / 1.14 ms.
+    if (b.type == GEOGCN_T_F32 && b.precision == GEOGCN_GEMM_BF16X3 && b.M >= kWholeRowsMin && b.K >= 192 && b.K <= 320 && b.N <= 1024)
         return backward_exact(ar, b, GEOGCN_GEMM_BF16X3, st);
     const int P = terms_of(b.type, b.precision), PX = b.X.type == GEOGCN_T_F32 ? P : 1;
     const int64_t plane = up(b.N, 64), ldo = P * plane;
@@ -1211,7 +1216,9 @@ int weight_grad_exact(Arena& ar, const WgradArgs& w, hipStream_t st) {
 }
 int weight_grad(Arena& ar, const WgradArgs& w, hipStream_t st) {
     if (w.precision == GEOGCN_GEMM_F32 && w.type == GEOGCN_T_F32) return weight_grad_exact(ar, w, st);
-    if (w.type == GEOGCN_T_F32 && w.precision == GEOGCN_GEMM_BF16X3 && tn_q8_takes(w.M, w.K, w.N)) {
+    // one narrow side: the operands are read once or twice, and terms in memory would cost more than the products (codes / terms: 440,000 x 300 x
+    // 256 249 / 577 us, 60,000 x 600 x 600 180 / 245, 20,000 x 300 x 2,048 104 / 182; but 20,000 x 1,024 x 1,024 196 / 183)
+    if (w.type == GEOGCN_T_F32 && w.precision == GEOGCN_GEMM_BF16X3 && std::min(w.K, w.N) <= 640 && std::max(w.K, w.N) <= 2048) {
         const float* B[1] = {static_cast<const float*>(w.dZ.p)};
         return tn_q8(ar, w.X, w.M, w.K, w.N, 1, B, w.dZ.ld, &w.dW, &w.lddw, st);
     }

@@ -1,6 +1,7 @@
 // 8-bit activation checkpoints: writing and reading them (format: mx8.h).
 // A training step keeps every layer's output until its backward; at 440,000 x 300 that is 528 MB a layer in fp32 and 145 MB in this form.
-// Both kernels are one pass over the data, bound by HBM: pack reads 4 (2) bytes a value and writes 1 + 1/32, unpack the reverse.
+// Both kernels are one pass over the data, bound by HBM: pack reads 4 (2) bytes a value and writes 1 + 1/32, unpack the reverse.  440,000 x 600 in
+// fp32: 0.31 and 0.27 ms for 1.33 GB each, 4.3 and 4.8 TB/s (a large copy: 4.6).
 #include "mx8.h"
 
 #include <algorithm>
@@ -8,7 +9,7 @@
 namespace geogcn {
 namespace {
 
-// A quad of columns per lane: 8 neighbouring lanes hold one block, whose maximum goes round them in three DPP-free shuffles; a wave covers
+// A quad of columns per lane: 8 neighbouring lanes hold one block, whose maximum goes round them in three shuffles; a wave covers
 // 8 blocks = 256 columns of a row and its stores (256 bytes of codes, 8 scale bytes) are contiguous.
 template <typename T>
 __global__ __launch_bounds__(256) void mx8_pack_kernel(int64_t n, int F, int qpr, const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ codes,

@@ -147,7 +147,7 @@ def test_saturated_gates(dev):
 
 
 BACKWARD = [(1, 1, 1), (1, 300, 300), (2, 33, 65), (5, 64, 64), (31, 129, 40), (64, 300, 33), (130, 40, 300), (300, 257, 129), (1000, 300, 930), (5000, 96, 161),
-            (4200, 300, 300), (700, 1100, 200), (16390, 300, 200), (16385, 129, 300), (17000, 400, 70)]
+            (4200, 300, 300), (700, 1100, 200), (16390, 300, 200), (16385, 129, 300), (16384, 192, 65), (17000, 400, 70)]
 
 
 def _check_bwd(dev, d, r, dH, kept, name, dtype, X=None, precision=None, need_dx=True, bias=True):
@@ -260,8 +260,11 @@ def test_empty_sizes(dev, dtype):
     x8 = ops.mx8_pack(z(0, 40))
     assert ops.mx8_unpack(x8).n == 0
     assert (ops.mx8_weight_grad(x8, z(0, 12), out=z(40, 12, 5.0)).t == 0).all()
-    H = ops.gated_dense(z(5, 0), z(0, 12), z(0, 12), bg=torch.full((12,), 2.0, device=dev), bu=torch.full((12,), 3.0, device=dev), act=ops.ACT_RELU)
-    assert (H.t[:, :12] == 6).all()                       # no inputs: the biases alone
+    for n in (5, 40):                                     # no inputs: the biases alone
+        H = ops.gated_dense(z(n, 0), z(0, 12), z(0, 12), bg=torch.full((12,), 2.0, device=dev), bu=torch.full((12,), 3.0, device=dev), act=ops.ACT_RELU)
+        assert (H.t[:, :12] == 6).all()
+    dX, dWg, _, dbg, dbu = ops.gated_dense_bwd(z(40, 12, 2.0), z(40, 0), z(0, 12), z(0, 12), ops.GatedTape(z(40, 12, 3.0), z(40, 12, 5.0)), act=ops.ACT_NONE, bias=True)
+    assert dX.F == 0 and dWg.n == 0 and (dbg[:12] == 40 * 10).all() and (dbu[:12] == 40 * 6).all()
 
 
 def _specials(n, F, seed):
@@ -304,7 +307,7 @@ def test_checkpoint_format(dev, n, F, dtype):
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16'])
-@pytest.mark.parametrize('M,K,N', [(1, 1, 1), (3, 33, 5), (40, 300, 129), (129, 64, 64), (1000, 300, 256), (5000, 200, 300), (300, 700, 1000), (16500, 300, 256), (20001, 33, 129), (16384, 320, 700)])
+@pytest.mark.parametrize('M,K,N', [(1, 1, 1), (3, 33, 5), (40, 300, 129), (129, 64, 64), (1000, 300, 256), (5000, 200, 300), (300, 700, 1000), (16500, 300, 256), (20001, 33, 129), (16384, 320, 700), (100, 900, 700), (2000, 640, 1300), (513, 2048, 40)])
 def test_weight_gradient_from_a_checkpoint(dev, M, K, N, dtype):
     from geographconv_amd import ops
     x8 = ops.mx8_pack(_mat(_rand((M, K), 1), dev, dtype))
