@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void terms_kernel(const TermsJobs jobs) {
 // ---- the tiled product ----------------------------------------------------------------------------------------------------------------------
 // C[m][n] = sum_k A . B over bf16 term planes.  An operand is stored along k (rows = its output dimension, "k-contiguous") or across it (rows =
 // k, "k-strided"): X is k-contiguous in the forward and k-strided in the weight gradient, W the other way round, so nothing is ever
-// transposed in memory.  Stages of BK k-values go straight from global memory to LDS (16 bytes a lane, double-buffered); a k-contiguous image is
+// transposed in memory.  Stages of BK k-values go straight from global memory to LDS (16 bytes a lane, two to six buffers); a k-contiguous image is
 // read as 16-byte fragments, a k-strided one through the transposing LDS read (4 k-values of a lane's own column).  Both images are
 // permuted in 16-byte pieces so that the lanes of a read phase meet different banks.
 // NSEG = 2: the block's columns are BN / 2 of B[0] and the same BN / 2 of B[1] -- a lane then owns g and u of one element.
