@@ -37,7 +37,8 @@ extern "C" {
  * geogcn_highway_bwd_f32 / _bf16s_f32 accept dHcarry = NULL.
  * 3: round 5: the fused highway launches take `precision` (GEOGCN_GEMM_F32 or GEOGCN_GEMM_BF16X3) before their workspace --
  * geogcn_gemm_dual_f32, geogcn_gemm_kcat_f32, geogcn_gemm_kcat_gated_f32, geogcn_gemm_kcat_gated_tanhbwd_f32 and the two
- * _workspace_bytes functions that size it (as their last argument); GEOGCN_GEMM_BF16X3 now also applies to transA = 1. */
+ * _workspace_bytes functions that size it (as their last argument); GEOGCN_GEMM_BF16X3 now also applies to transA = 1.
+ * Added since without a version change: geogcn_gated_fwd, geogcn_gated_bwd, geogcn_mx8_pack, geogcn_mx8_unpack, geogcn_mx8_weight_grad. */
 #define GEOGCN_ABI_VERSION 3
 
 #define GEOGCN_E_NULL   (-1)   /* required pointer is NULL            */
@@ -509,7 +510,8 @@ int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, 
  * type: GEOGCN_T_F32 or GEOGCN_T_BF16, that of every matrix; bg, bu: fp32, may be NULL (each on its own).  Products of fp32 matrices:
  * GEOGCN_GEMM_F32 (the exact fp32 kernels, in launches of their own), GEOGCN_GEMM_BF16X3 (three bf16 terms a value, fp32-class) or
  * GEOGCN_GEMM_BF16 (operands rounded to bf16); accumulation fp32.  (An infinity is not the sum of three bf16 terms: under BF16X3 its row
- * gives NaN.)  Products of bf16 matrices are one kind, whatever `precision` says.
+ * gives NaN.)  Calls of up to 16 rows multiply in plain fp32 under either of the first two.  Products of bf16 matrices are one kind, whatever
+ * `precision` says.
  * keep: what of G = X.Wg + bg and U = X.Wu + bu is stored for the backward -- nothing, in the block's type (pitch >= H's), or as 8-bit
  * checkpoints (codes G / U with pitch ldg / ldu and scales Gs / Us as geogcn_mx8_pack writes them).
  * K, N <= 2^20, pitches <= 2^21.  H, G, U, dX, dWg, dWu overlap none of the other matrices.

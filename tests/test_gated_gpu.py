@@ -232,6 +232,28 @@ def test_pitches_junk_pads_and_neighbouring_rows(dev, dtype):
            _forward_bounds(dict(r, bg=np.zeros(N)), 'silu', dtype)[0], 'one bias')
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('M', [9, 200, 16400])
+def test_a_row_that_is_not_finite_stays_alone(dev, M, dtype):
+    """An infinity or a NaN in a row of X reaches that row of H, G and U and no other; checkpoint blocks of the other rows are untouched too."""
+    from geographconv_amd import ops
+    d, _ = _problem(dev, M, 70, 100, dtype, True, 6)
+    args = (d['Wg'], d['Wu'], d['bg'], d['bu'])
+    want, kept = ops.gated_dense(d['X'], *args, act=ops.ACT_SILU, keep='full')
+    want8, kept8 = ops.gated_dense(d['X'], *args, act=ops.ACT_SILU, keep='mx8')
+    bad = [3, 8]
+    d['X'].t[3, 5] = float('inf')
+    d['X'].t[8, 69] = float('nan')
+    got, gk = ops.gated_dense(d['X'], *args, act=ops.ACT_SILU, keep='full')
+    got8, gk8 = ops.gated_dense(d['X'], *args, act=ops.ACT_SILU, keep='mx8')
+    ok = torch.ones(M, dtype=torch.bool, device=dev)
+    ok[bad] = False
+    for a, b in ((want.t, got.t), (kept.G.t, gk.G.t), (kept.U.t, gk.U.t), (want8.t, got8.t), (kept8.G.codes, gk8.G.codes), (kept8.U.scales, gk8.U.scales)):
+        assert torch.equal(a[ok], b[ok])
+    assert not torch.isfinite(got.t[bad, :100].float()).any() and torch.isnan(got.t[8, :100].float()).all()
+    assert not torch.isfinite(ops.mx8_unpack(gk8.G).t[bad, :100].float()).any()
+
+
 def test_outputs_that_overlap_operands_are_refused(dev):
     from geographconv_amd import ops
     d, _ = _problem(dev, 20, 32, 32, 'f32', True, 1)
