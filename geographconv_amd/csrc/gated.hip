@@ -293,6 +293,12 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
             _Pragma("unroll") for (int j = 0; j < JN; ++j) GEOGCN_MFMA(A_, B_, J0, i, j, 0, 0)                                         \
             REFILL(i, 0)                                                                                                               \
         }                                                                                                                              \
+    } else if constexpr (PA == 2) {                                                                                                    \
+        GEOGCN_TERM(A_, B_, J0, JN, 1, 0) _Pragma("unroll") for (int i = 0; i < MT; ++i) { REFILL(i, 1) }                                  \
+        _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                               \
+            _Pragma("unroll") for (int j = 0; j < JN; ++j) GEOGCN_MFMA(A_, B_, J0, i, j, 0, 0)                                         \
+            REFILL(i, 0)                                                                                                               \
+        }                                                                                                                              \
     } else {                                                                                                                           \
         _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                               \
             _Pragma("unroll") for (int pb = PB - 1; pb >= 0; --pb) _Pragma("unroll") for (int j = 0; j < JN; ++j) GEOGCN_MFMA(A_, B_, J0, i, j, 0, pb) \
@@ -303,6 +309,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
 #define GEOGCN_REFILL(i, p) fa[i][p] = IA::read(la + at + (uint32_t)((p) * IA::kBytes), wm * MT + i, 0, lg);
     constexpr bool BYK = BK == 64;
     static_assert(BK == 32 || (PA == 1 && PB == 1), "two k-steps a stage: one term");
+    static_assert(PA == PB || PA == 1 || (PA == 2 && PB == 1), "cross products");
     constexpr int N0 = BYK ? NT : (NT + 1) / 2, N1 = BYK ? NT : NT - N0, J1 = BYK ? 0 : N0;       // columns of the two phases, in tiles
     bf16x8 fa[MT][PA], fa1[BYK ? MT : 1][PA], b0[N0][PB], b1[N1][PB];
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
@@ -899,6 +906,12 @@ int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
                                  {256, 128, 64, 3, 1, 0.85, run_tiles<1, 1, false, false, 1, 256, 128, 64, 4, 2, 3, false>},
                                  {128, 128, 64, 2, 2, 0.8, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 2, false>},
                                  {128, 128, 64, 4, 1, 0.75, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 4, false>}};
+    // dG, dU of a bf16 block as two terms (256 x 256 / 256 x 128 / 128 x 128: 8,192 x 1,024 -> 4,096 251 / 277 / 282 us, 60,000 x 600 -> 600
+    // 214 / 250 / 238, 1,000 x 600 -> 600 30 / 23 / 19)
+    static const Shape two[] = {{256, 256, 32, 3, 1, 1.0, run_tiles<2, 1, false, false, 1, 256, 256, 32, 2, 4, 3, false>},
+                                {256, 128, 32, 3, 1, 0.82, run_tiles<2, 1, false, false, 1, 256, 128, 32, 4, 2, 3, false>},
+                                {128, 128, 32, 2, 2, 0.78, run_tiles<2, 1, false, false, 1, 128, 128, 32, 2, 4, 2, false>}};
+    if (P == 2) return run_best(two, ar, t, t.ncols, 1, 2, st);
     return P == 3 ? run_best(fp32, ar, t, t.ncols, 1, 6, st) : run_best(bf16, ar, t, t.ncols, 1, 1, st);
 }
 
@@ -910,11 +923,16 @@ int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_
     static const Shape bf16[] = {{128, 128, 64, 3, 1, 1.0, run_tiles<1, 1, true, true, 2, 128, 256, 64, 2, 4, 3, false>},
                                  {128, 64, 64, 2, 2, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 2, 2, false>},
                                  {128, 64, 64, 4, 1, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 4, 4, false>}};
+    // dG, dU of a bf16 block as two terms (128 / 64 columns of each, with the gate pass: 8,192 x 1,024 -> 4,096 330 / 362 us, 4,097 x 1,024 ->
+    // 1,536 91 / 88, 440,000 x 300 -> 300 882 / 843)
+    static const Shape two[] = {{128, 128, 32, 3, 1, 1.0, run_tiles<1, 2, true, true, 2, 128, 256, 32, 2, 4, 3, false>},
+                                {128, 64, 32, 2, 2, 0.8, run_tiles<1, 2, true, true, 2, 128, 128, 32, 2, 4, 2, false>}};
     static const Shape mx8_one[] = {{160, 256, 32, 2, 1, 1.0, run_tiles<1, 3, true, true, 1, 160, 256, 32, 2, 4, 2, false>},
                                     {128, 128, 32, 5, 1, 0.8, run_tiles<1, 3, true, true, 1, 128, 128, 32, 2, 4, 5, false>}};
     static const Shape bf16_one[] = {{128, 128, 32, 6, 1, 1.0, run_tiles<1, 1, true, true, 1, 128, 128, 32, 2, 4, 6, false>}};
     if (nseg == 2) {
         if (PA == 3) return run_best(fp32, ar, t, t.ncols, 2, 6, st);
+        if (PB == 2) return run_best(two, ar, t, t.ncols, 2, 2, st);
         return PB == 3 ? run_best(mx8, ar, t, t.ncols, 2, 3, st) : run_best(bf16, ar, t, t.ncols, 2, 1, st);
     }
     return PB == 3 ? run_best(mx8_one, ar, t, t.ncols, 1, 3, st) : run_best(bf16_one, ar, t, t.ncols, 1, 1, st);
@@ -951,6 +969,9 @@ bool act_ok(int act) {
 
 // terms per value of an operand: bf16 and 8-bit values are one term; fp32 three, or one (rounded) where the caller asked for bf16 products
 int terms_of(int type, int precision) { return type == GEOGCN_T_F32 && precision != GEOGCN_GEMM_BF16 ? 3 : 1; }
+// ... of dG and dU, which are formed in fp32 whatever the block's type: in a bf16 block two (2^-16 of a value; one would add 2^-8 of every
+// product to results that are rounded to 2^-8 once: 0.0023 from the 64-bit results in the norm, 0.0017 with two) unless bf16 products are asked for
+int grad_terms_of(int type, int precision) { return precision == GEOGCN_GEMM_BF16 ? 1 : type == GEOGCN_T_F32 ? 3 : 2; }
 
 int check_dims(const char* who, int64_t M, int64_t K, int64_t N) {
     GEOGCN_REQUIRE(M >= 0 && K >= 0 && N >= 0, GEOGCN_E_SIZE, "%s: negative size", who);
@@ -1080,7 +1101,7 @@ int gate_gradients(Arena& ar, const BwdArgs& b, int P, int64_t ldo, hipStream_t 
         const dim3 grid((unsigned)cblocks, (unsigned)nparts);
         const bool f32 = b.type == GEOGCN_T_F32, q8 = b.G.type == GEOGCN_T_MX8;
         constexpr int F = GEOGCN_T_F32, H = GEOGCN_T_BF16, Q = GEOGCN_T_MX8;
-        auto* k = !f32 ? (q8 ? &gate_grad_kernel<1, H, Q> : &gate_grad_kernel<1, H, H>)
+        auto* k = !f32 ? (P == 2 ? (q8 ? &gate_grad_kernel<2, H, Q> : &gate_grad_kernel<2, H, H>) : (q8 ? &gate_grad_kernel<1, H, Q> : &gate_grad_kernel<1, H, H>))
                   : P == 3 ? (q8 ? &gate_grad_kernel<3, F, Q> : &gate_grad_kernel<3, F, F>)
                   : P == 1 ? (q8 ? &gate_grad_kernel<1, F, Q> : &gate_grad_kernel<1, F, F>)
                            : (q8 ? &gate_grad_kernel<0, F, Q> : &gate_grad_kernel<0, F, F>);
@@ -1161,10 +1182,10 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
     // 600 1.40 / 1.14 ms.
     if (b.type == GEOGCN_T_F32 && b.precision == GEOGCN_GEMM_BF16X3 && b.M >= kWholeRowsMin && b.K >= 192 && b.K <= 320 && b.N <= 1024)
         return backward_exact(ar, b, GEOGCN_GEMM_BF16X3, st);
-    const int P = terms_of(b.type, b.precision), PX = b.X.type == GEOGCN_T_F32 ? P : 1;
-    const int64_t plane = up(b.N, 64), ldo = P * plane;
+    const int P = terms_of(b.type, b.precision), PX = b.X.type == GEOGCN_T_F32 ? P : 1, PG = grad_terms_of(b.type, b.precision);
+    const int64_t plane = up(b.N, 64), ldo = PG * plane;
     uint16_t *dG, *dU;
-    if (const int rc = gate_gradients(ar, b, P, plane, st, &dG, &dU)) return rc;
+    if (const int rc = gate_gradients(ar, b, PG, plane, st, &dG, &dU)) return rc;
     TermsJobs jobs{};
     Planes wg{}, wu{}, x{};
     if (b.dX) {
@@ -1187,7 +1208,7 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
         t.B[1] = wu.p; t.ldb[1] = wu.ld; t.planeB[1] = wu.plane;
         for (int q = 0; q < 2; ++q) { t.lda[q] = ldo; t.planeA[q] = plane; }
         t.out_type = b.type; t.C[0] = b.dX; t.ldc[0] = b.lddx; t.ncols = out_cols(b.type, b.K, b.lddx);
-        if (const int rc = run_input_grad(ar, t, P, st)) return rc;
+        if (const int rc = run_input_grad(ar, t, PG, st)) return rc;
     }
     if (b.dW[0]) {
         TileArgs t = tile_args();
@@ -1198,7 +1219,7 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
         t.out_type = b.type;
         t.ncols = std::max(out_cols(b.type, b.N, b.lddw[0]), out_cols(b.type, b.N, b.lddw[1]));
         if (b.lddw[0] != b.lddw[1]) t.ncols = std::min(out_cols(b.type, b.N, b.lddw[0]), out_cols(b.type, b.N, b.lddw[1]));
-        if (const int rc = run_weight_grad(ar, t, PX, P, 2, st)) return rc;
+        if (const int rc = run_weight_grad(ar, t, PX, PG, 2, st)) return rc;
     }
     return 0;
 }

@@ -44,14 +44,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {          // 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// four consecutive values x -> their P bf16 terms (P = 3: x = x1 + x2 + x3 exactly, the residuals are exact in fp32; P = 1: rounded)
+// four consecutive values x -> their P bf16 terms (P = 3: x = x1 + x2 + x3 exactly, the residuals are exact in fp32; P = 2: to 2^-16 of x; P = 1:
+// rounded)
 template <int P>
 __device__ __forceinline__ void bf16_terms4(const float4& x, uint2 (&t)[P]) {
     t[0] = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-    if constexpr (P == 3) {
+    if constexpr (P >= 2) {
         const float r0 = x.x - bf16_lo(t[0].x), r1 = x.y - bf16_hi(t[0].x), r2 = x.z - bf16_lo(t[0].y), r3 = x.w - bf16_hi(t[0].y);
         t[1] = make_uint2(pack_bf16(r0, r1), pack_bf16(r2, r3));
-        t[2] = make_uint2(pack_bf16(r0 - bf16_lo(t[1].x), r1 - bf16_hi(t[1].x)), pack_bf16(r2 - bf16_lo(t[1].y), r3 - bf16_hi(t[1].y)));
+        if constexpr (P == 3) t[2] = make_uint2(pack_bf16(r0 - bf16_lo(t[1].x), r1 - bf16_hi(t[1].x)), pack_bf16(r2 - bf16_lo(t[1].y), r3 - bf16_hi(t[1].y)));
     }
 }
 

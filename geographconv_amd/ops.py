@@ -1352,7 +1352,7 @@ def mx8_weight_grad(X: MX8Mat, dZ, out=None, precision=None):
     if dZ.n != X.n or X.bf16 != bf16:
         raise ValueError("mx8_weight_grad: the checkpoint (%d rows, %s) and dZ (%d rows, %s) do not match"
                          % (X.n, 'bf16' if X.bf16 else 'fp32', dZ.n, 'bf16' if bf16 else 'fp32'))
-    prec = _block_precision(precision, bf16)
+    prec = _block_precision(precision)
     out = _new_like_block(bf16, X.F, dZ.F, X.device) if out is None else _check_out(out, X.F, dZ.F, HMat if bf16 else DMat, 'mx8_weight_grad: the output')
     _on_device(_same_device(X, dZ, out), _call_with_ws, _ffi.lib().geogcn_mx8_weight_grad, 'mx8_weight_grad', X.n, X.F, dZ.F, _mat_type(dZ),
                *_mat_args(X), dZ.t.data_ptr(), dZ.ld, out.t.data_ptr(), out.ld, prec)
@@ -1363,12 +1363,12 @@ _KEEP = {None: _ffi.KEEP_NONE, 'full': _ffi.KEEP_FULL, 'mx8': _ffi.KEEP_MX8}
 GATED_ACTS = (ACT_NONE, ACT_TANH, ACT_SIGMOID, ACT_RELU, ACT_SILU, ACT_GELU)
 
 
-def _block_precision(precision, bf16):
-    """-> GEMM_* of the block's products: a bf16 block has one kind; an fp32 one follows `precision` (None: the default)."""
+def _block_precision(precision):
+    """-> GEMM_* of the block's products (None: the default)."""
     p = precision or GEMM_PRECISION
     if p not in GEMM_PRECISIONS:
         raise ValueError("unknown precision %r" % (precision,))
-    return _ffi.GEMM_BF16 if bf16 else GEMM_PRECISIONS[p]
+    return GEMM_PRECISIONS[p]
 
 
 def _check_gated(X, Wg, Wu, act, who):
@@ -1399,7 +1399,7 @@ def gated_dense(X, Wg, Wu, bg: torch.Tensor = None, bu: torch.Tensor = None, act
     bf16, M, K, N = _check_gated(X, Wg, Wu, act, 'gated_dense')
     _check_vec(bg, N, 'gated_dense: bg')
     _check_vec(bu, N, 'gated_dense: bu')
-    prec = _block_precision(precision, bf16)
+    prec = _block_precision(precision)
     kind = HMat if bf16 else DMat
     H = _new_like_block(bf16, M, N, X.device) if out is None else _check_out(out, M, N, kind, 'gated_dense: the output')
     index = _same_device(X, Wg, Wu, bg, bu, H)
@@ -1422,7 +1422,8 @@ def gated_dense_bwd(dH, X, Wg, Wu, kept: GatedTape, act=ACT_SIGMOID, dX=None, dW
                     dbu: torch.Tensor = None, bias=False, need_input_grad=True, precision=None):
     """-> (dX, dWg, dWu, dbg, dbu) of gated_dense from the gradient dH of its result, its input X and the kept G, U -- X and `kept` each
     dense or in 8 bits (MX8Mat).  The gradient buffers may be given; `bias` (or a given dbg / dbu pair) asks for the bias gradients,
-    `need_input_grad=False` leaves dX out (None comes back).  `act` and `precision` must be the forward's."""
+    `need_input_grad=False` leaves dX out (None comes back).  `act` must be the forward's.  `precision`: as the forward's; in a bf16 block
+    'bf16' rounds dG and dU to bf16 before the products (2^-8 of each), 'bf16x3' and 'f32' multiply them as two bf16 terms (2^-16)."""
     bf16, M, K, N = _check_gated(X, Wg, Wu, act, 'gated_dense_bwd')
     kind = HMat if bf16 else DMat
     _check_out(dH, M, N, kind, 'gated_dense_bwd: dH')
@@ -1434,7 +1435,7 @@ def gated_dense_bwd(dH, X, Wg, Wu, kept: GatedTape, act=ACT_SIGMOID, dX=None, dW
     for m, n, F, what in ((dX, M, K, 'dX'), (dWg, K, N, 'dWg'), (dWu, K, N, 'dWu')):
         if m is not None:
             _check_out(m, n, F, kind, 'gated_dense_bwd: ' + what)
-    prec = _block_precision(precision, bf16)
+    prec = _block_precision(precision)
     index, dev = _same_device(dH, X, Wg, Wu, kept.G, kept.U, dX, dWg, dWu, dbg, dbu), dH.device
     if dX is not None or dWg is not None or dbg is not None:
         _check_apart('gated_dense_bwd', [dX, dWg, dWu, dbg, dbu], [dH, X, Wg, Wu, kept.G, kept.U])

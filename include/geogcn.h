@@ -510,8 +510,8 @@ int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, 
  * type: GEOGCN_T_F32 or GEOGCN_T_BF16, that of every matrix; bg, bu: fp32, may be NULL (each on its own).  Products of fp32 matrices:
  * GEOGCN_GEMM_F32 (the exact fp32 kernels, in launches of their own), GEOGCN_GEMM_BF16X3 (three bf16 terms a value, fp32-class) or
  * GEOGCN_GEMM_BF16 (operands rounded to bf16); accumulation fp32.  (An infinity is not the sum of three bf16 terms: under BF16X3 its row
- * gives NaN.)  Calls of up to 16 rows multiply in plain fp32 under either of the first two.  Products of bf16 matrices are one kind, whatever
- * `precision` says.
+ * gives NaN.)  Calls of up to 16 rows multiply in plain fp32 under either of the first two.  The forward products of bf16 matrices are exact
+ * products accumulated in fp32, whatever `precision` says.
  * keep: what of G = X.Wg + bg and U = X.Wu + bu is stored for the backward -- nothing, in the block's type (pitch >= H's), or as 8-bit
  * checkpoints (codes G / U with pitch ldg / ldu and scales Gs / Us as geogcn_mx8_pack writes them).
  * K, N <= 2^20, pitches <= 2^21.  H, G, U, dX, dWg, dWu overlap none of the other matrices.
@@ -526,8 +526,9 @@ int geogcn_gated_fwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* 
                      uint8_t* Gs, void* U, int64_t ldu, uint8_t* Us, int32_t precision, void* ws, size_t* ws_bytes, void* stream);
 /* Its backward from dH, X and the kept G, U (x_type / kept_type: the block's type or GEOGCN_T_MX8 with scales Xs / Gs, Us):
  *   dG = dH * U * act'(G), dU = dH * act(G);  dX = dG.Wg^T + dU.Wu^T;  dWg = X^T.dG, dWu = X^T.dU;  dbg, dbu = column sums (fp32).
- * dX, the pair dWg / dWu and the pair dbg / dbu may each be NULL (not formed).  In a bf16 block dG and dU are rounded to bf16 before the
- * products, not before the bias gradients.  ws: as above.                                                                                 */
+ * dX, the pair dWg / dWu and the pair dbg / dbu may each be NULL (not formed).  In a bf16 block dG and dU are formed in fp32 and multiplied as
+ * two bf16 terms each (2^-16 of a value; one that is not finite gives NaN) under GEOGCN_GEMM_F32 and GEOGCN_GEMM_BF16X3, rounded to bf16
+ * (2^-8) under GEOGCN_GEMM_BF16; the bias gradients are sums of the fp32 values under all three.  ws: as above.                           */
 int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* dH, int64_t lddh, int32_t x_type, const void* X, int64_t ldx,
                      const uint8_t* Xs, const void* Wg, int64_t ldwg, const void* Wu, int64_t ldwu, int32_t kept_type, const void* G, int64_t ldg,
                      const uint8_t* Gs, const void* U, int64_t ldu, const uint8_t* Us, int32_t act, void* dX, int64_t lddx, void* dWg,
