@@ -1,8 +1,9 @@
 // The 8-bit checkpoint format, shared by the kernels that write it and the ones that read it.
 // 32 consecutive values of a row share one power-of-two scale 2^s, stored as the byte s + 127; a value is the e4m3 code of x / 2^s (4
 // significant bits, round to nearest even).  s is the smallest exponent, -126 at least, with max|x| <= 448 * 2^s (448 = the largest e4m3
-// value): no value saturates, so every rounding is off by at most half a step, and the division is exact.  A block that holds an infinity
-// or a NaN has the byte 255 and stands for NaN throughout.
+// value): no value saturates, so every rounding is off by at most half a step, and the division is exact.  At the largest scale, 2^120, the
+// code 256 would stand for 2^128, which is no fp32 number: values from 248 * 2^120 on take the code 240 below it (off by 2^-4 of themselves
+// at most, like any other).  A block that holds an infinity or a NaN has the byte 255 and stands for NaN throughout.
 #pragma once
 #include "common.h"
 
@@ -24,7 +25,9 @@ __device__ __forceinline__ float mx8_scale(uint32_t byte) { return __uint_as_flo
 
 __device__ __forceinline__ uint32_t mx8_encode4(float x0, float x1, float x2, float x3, float inv, bool finite) {
     // (0 * inf of a NaN block would be NaN: the codes of such a block are written as 0)
-    const float y0 = finite ? x0 * inv : 0.f, y1 = finite ? x1 * inv : 0.f, y2 = finite ? x2 * inv : 0.f, y3 = finite ? x3 * inv : 0.f;
+    const float top = inv == 0x1p-120f ? 240.f : 448.f;
+    const auto code = [&](float x) { return finite ? __builtin_amdgcn_fmed3f(x * inv, -top, top) : 0.f; };
+    const float y0 = code(x0), y1 = code(x1), y2 = code(x2), y3 = code(x3);
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(y2, y3, w, true);
     return (uint32_t)w;

@@ -498,7 +498,8 @@ int geogcn_reg_penalty_f32(int64_t n, const float* p, const float* regmask, floa
 /* ---- 8-bit activation checkpoints (no reference counterpart: the reference keeps fp32 activations) -------------------------------
  * A row's values are taken in blocks of 32 that share a scale 2^s, s the smallest exponent (-126 at least) with max|x| <= 448 * 2^s, stored as
  * the byte s + 127 in scale[n x ldq / 32]; codes[n x ldq] holds e4m3 codes of x / 2^s, round to nearest even (codes behind column F are 0).
- * No value saturates.  A block with an infinity or a NaN has the scale byte 255 and reads back as NaN throughout.  type: that of X / Y
+ * No value saturates, but for those from 1.9375 * 2^127 on, which read back as 1.875 * 2^127 (the next code is no fp32 number).  A block with
+ * an infinity or a NaN has the scale byte 255 and reads back as NaN throughout.  type: that of X / Y
  * (GEOGCN_T_F32 or GEOGCN_T_BF16).  ldx % 4 == 0, ldq % 32 == 0, ldq >= F; X / Y aligned to 16 (fp32) / 8 (bf16) bytes, codes to 4.
  * unpack writes the pad columns of Y (roundup4 / roundup64, never past the pitch) as zero.                                                */
 int geogcn_mx8_pack(int64_t n, int32_t F, int32_t type, const void* X, int64_t ldx, uint8_t* codes, int64_t ldq, uint8_t* scale, void* stream);

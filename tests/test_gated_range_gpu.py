@@ -40,3 +40,39 @@ def test_bf16_gradients_are_rounded_once(dev, M, K, N, eight):
         res = ops.gated_dense_bwd(dH, X, d['Wg'], d['Wu'], ops.GatedTape(G, U), act=ops.ACT_SILU, precision=precision)
         for m, (name, (w, mag, e)) in zip(res, want.items()):
             _check(_f64(m), (w, (1 + BF) * ((ENV + terms) * mag + 2 * e) + BF * np.abs(w) + 1e-30), '%s %s' % (name, precision))
+
+
+TOP = 240 * 2.0 ** 120          # the largest number that a checkpoint of finite values stands for: the next code at this scale is 2^128
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_the_largest_values_stay_finite(dev, dtype):
+    """Finite values up to the type's largest read back finite, off by 2^-4 of themselves at most, their block's other values too."""
+    from geographconv_amd import ops
+    big = torch.finfo(torch.float32 if dtype == 'f32' else torch.bfloat16).max
+    x = np.zeros((4, 64))
+    x[0, :6] = [big, -big, 3.3e38, 1.9375 * 2.0 ** 127, 2.0 ** 127, 2.0 ** 125]
+    x[1, :3] = [1.875 * 2.0 ** 127, -1.75 * 2.0 ** 127, 1.5 * 2.0 ** 118]
+    x[2, 33:35] = [-1.9375 * 2.0 ** 127, 3e37]
+    x[3] = big
+    m = _mat(x.astype(np.float32), dev, dtype)
+    q = ops.mx8_pack(m)
+    x = _f64(m)
+    got = _f64(ops.mx8_unpack(q))
+    s = 2.0 ** (np.repeat(q.scales.cpu().numpy().astype(np.float64), 32, axis=1) - 127)
+    _check(got, (x, np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * s)), 'checkpoint')
+    want = np.clip(R.mx8(x)[2], -TOP, TOP)
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize('M,K', [(1, 1), (5, 40), (300, 40), (40, 4096)])
+def test_the_largest_pre_activations_stay_finite_in_their_checkpoints(dev, M, K):
+    """... in the checkpoints that the block's forward writes: a few rows, tiles, a split reduction."""
+    from geographconv_amd import ops
+    big = float(torch.finfo(torch.bfloat16).max)
+    X, Wg, Wu = np.zeros((M, K), np.float32), np.zeros((K, 40), np.float32), np.zeros((K, 40), np.float32)
+    X[:, 0] = 1
+    Wg[0, ::3], Wg[0, 1::3], Wu[0] = big, -2.0 ** 126, 0.5
+    _, kept = ops.gated_dense(*(_mat(a, dev, 'bf16') for a in (X, Wg, Wu)), act=ops.ACT_NONE, keep='mx8')
+    got = _f64(ops.mx8_unpack(kept.G))
+    assert np.array_equal(got, np.tile(np.clip(R.mx8(Wg[:1].astype(np.float64))[2], -TOP, TOP), (M, 1)))
