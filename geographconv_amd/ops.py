@@ -1265,13 +1265,14 @@ def _same_device(first, *rest):
 
 
 def _check_apart(who, outs, ins):
-    """Given outputs overlap neither each other nor an operand (they are written while operands are still read)."""
-    def span(m):
-        t = _tensor(m)
-        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-    spans = [(o, *span(o)) for o in outs if o is not None]
-    for i, (o, a, b) in enumerate(spans):
-        for _, c, d in [(None, *span(m)) for m in ins if m is not None] + spans[:i]:
+    """Given outputs overlap neither each other nor an operand (they are written while operands are still read); a checkpoint is its codes and
+    its scales."""
+    def spans(ms):
+        ts = [t for m in ms if m is not None for t in ((m.codes, m.scales) if isinstance(m, MX8Mat) else (_tensor(m),))]
+        return [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel()]
+    written, read = spans(outs), spans(ins)
+    for i, (a, b) in enumerate(written):
+        for c, d in read + written[:i]:
             if a < d and c < b:
                 raise ValueError("%s: an output overlaps another operand" % who)
 
@@ -1325,6 +1326,8 @@ def mx8_pack(X, out: MX8Mat = None):
         out = MX8Mat.empty(X.n, X.F, X.device, bf16)
     elif (out.n, out.F, out.bf16) != (X.n, X.F, bf16):
         raise ValueError("mx8_pack: the output does not have the input's shape and type")
+    else:
+        _check_apart('mx8_pack', [out], [X])
     _on_device(_same_device(X, out), _call, _ffi.lib().geogcn_mx8_pack, 'mx8_pack', X.n, X.F, t, X.t.data_ptr(), X.ld, out.codes.data_ptr(), out.ld,
                out.scales.data_ptr())
     return out
@@ -1336,7 +1339,10 @@ def mx8_unpack(Q: MX8Mat, out=None):
     if _mat_type(Q) != _ffi.T_MX8:
         raise ValueError("mx8_unpack: not an 8-bit checkpoint")
     kind = HMat if Q.bf16 else DMat
-    out = _new_like_block(Q.bf16, Q.n, Q.F, Q.device) if out is None else _check_out(out, Q.n, Q.F, kind, 'mx8_unpack: the output')
+    if out is None:
+        out = _new_like_block(Q.bf16, Q.n, Q.F, Q.device)
+    else:
+        _check_apart('mx8_unpack', [_check_out(out, Q.n, Q.F, kind, 'mx8_unpack: the output')], [Q])
     _on_device(_same_device(Q, out), _call, _ffi.lib().geogcn_mx8_unpack, 'mx8_unpack', Q.n, Q.F, _mat_type(out), Q.codes.data_ptr(), Q.ld,
                Q.scales.data_ptr(), out.t.data_ptr(), out.ld)
     return out
@@ -1345,7 +1351,7 @@ def mx8_unpack(Q: MX8Mat, out=None):
 @_timed('mx8_weight_grad')
 def mx8_weight_grad(X: MX8Mat, dZ, out=None, precision=None):
     """X^T . dZ with X kept in 8 bits: the weight gradient of a dense layer from its checkpointed input.  `precision`: 'bf16x3'
-    (fp32-class), 'bf16', or 'f32' (the checkpoint is read back and the exact fp32 kernel multiplies)."""
+    (fp32-class), 'bf16', or 'f32' (the checkpoint is read back and the exact fp32 kernel multiplies).  `out` overlaps no operand."""
     if _mat_type(X) != _ffi.T_MX8 or _mat_type(dZ) == _ffi.T_MX8:
         raise ValueError("mx8_weight_grad takes an 8-bit checkpoint and a dense gradient")
     bf16 = isinstance(dZ, HMat)
@@ -1353,7 +1359,10 @@ def mx8_weight_grad(X: MX8Mat, dZ, out=None, precision=None):
         raise ValueError("mx8_weight_grad: the checkpoint (%d rows, %s) and dZ (%d rows, %s) do not match"
                          % (X.n, 'bf16' if X.bf16 else 'fp32', dZ.n, 'bf16' if bf16 else 'fp32'))
     prec = _block_precision(precision)
-    out = _new_like_block(bf16, X.F, dZ.F, X.device) if out is None else _check_out(out, X.F, dZ.F, HMat if bf16 else DMat, 'mx8_weight_grad: the output')
+    if out is None:
+        out = _new_like_block(bf16, X.F, dZ.F, X.device)
+    else:
+        _check_apart('mx8_weight_grad', [_check_out(out, X.F, dZ.F, HMat if bf16 else DMat, 'mx8_weight_grad: the output')], [X, dZ])
     _on_device(_same_device(X, dZ, out), _call_with_ws, _ffi.lib().geogcn_mx8_weight_grad, 'mx8_weight_grad', X.n, X.F, dZ.F, _mat_type(dZ),
                *_mat_args(X), dZ.t.data_ptr(), dZ.ld, out.t.data_ptr(), out.ld, prec)
     return out

@@ -501,7 +501,7 @@ int geogcn_reg_penalty_f32(int64_t n, const float* p, const float* regmask, floa
  * No value saturates, but for those from 1.9375 * 2^127 on, which read back as 1.875 * 2^127 (the next code is no fp32 number).  A block with
  * an infinity or a NaN has the scale byte 255 and reads back as NaN throughout.  type: that of X / Y
  * (GEOGCN_T_F32 or GEOGCN_T_BF16).  ldx % 4 == 0, ldq % 32 == 0, ldq >= F; X / Y aligned to 16 (fp32) / 8 (bf16) bytes, codes to 4.
- * unpack writes the pad columns of Y (roundup4 / roundup64, never past the pitch) as zero.                                                */
+ * unpack writes the pad columns of Y (roundup4 / roundup64, never past the pitch) as zero.  What is written overlaps nothing that is read.   */
 int geogcn_mx8_pack(int64_t n, int32_t F, int32_t type, const void* X, int64_t ldx, uint8_t* codes, int64_t ldq, uint8_t* scale, void* stream);
 int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, int64_t ldq, const uint8_t* scale, void* Y, int64_t ldy,
                       void* stream);
@@ -535,7 +535,7 @@ int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, const void* 
                      const uint8_t* Gs, const void* U, int64_t ldu, const uint8_t* Us, int32_t act, void* dX, int64_t lddx, void* dWg,
                      int64_t lddwg, void* dWu, int64_t lddwu, float* dbg, float* dbu, int32_t precision, void* ws, size_t* ws_bytes, void* stream);
 /* dW [K x N] = X^T.dZ of a dense layer whose input X [M x K] was kept as an 8-bit checkpoint (type: that of dZ and dW).  A checkpointed value is
- * one bf16 term: three cross products a value of fp32 dZ instead of six.  ws: as above.                                                    */
+ * one bf16 term: three cross products a value of fp32 dZ instead of six.  dW overlaps none of the others.  ws: as above.                   */
 int geogcn_mx8_weight_grad(int64_t M, int64_t K, int64_t N, int32_t type, const uint8_t* X, int64_t ldx, const uint8_t* Xs, const void* dZ,
                            int64_t lddz, void* dW, int64_t lddw, int32_t precision, void* ws, size_t* ws_bytes, void* stream);
 

@@ -1,0 +1,47 @@
+"""Calls of the gated dense block and the 8-bit checkpoints that are turned down on the host, and what their sources state (no GPU)."""
+import pytest
+import torch
+
+from geographconv_amd import ops
+
+from .test_gated import D, Hm, Q
+
+
+def _shared(n, F, kind):
+    """-> a dense matrix and a checkpoint in one piece of memory: the matrix' last row holds the checkpoint's scales (or codes)"""
+    w = (F + 31) // 32
+    if kind == 'scales':
+        ld = max(ops.pad4(F), (n * w + 3) // 4 * 4)
+        raw = torch.zeros(n * ld * 4, dtype=torch.uint8)
+        scales = raw[(n - 1) * ld * 4:][:n * w].view(n, w)
+        codes = torch.zeros(n, 32 * w, dtype=torch.uint8)
+    else:
+        ld = max(ops.pad4(F), 8 * w * n)
+        raw = torch.zeros(n * ld * 4, dtype=torch.uint8)
+        codes = raw[(n - 1) * ld * 4:][:n * 32 * w].view(n, 32 * w)
+        scales = torch.zeros(n, w, dtype=torch.uint8)
+    return ops.DMat(n, F, t=raw.view(torch.float32).view(n, ld)), ops.MX8Mat(n, F, codes, scales)
+
+
+@pytest.mark.parametrize('kind', ['codes', 'scales'])
+def test_overlapping_outputs_of_the_checkpoint_calls_are_refused(kind):
+    m, q = _shared(4, 40, kind)
+    z = D(4, 40)
+    for call in (lambda: ops.mx8_pack(m, out=q), lambda: ops.mx8_unpack(q, out=m)):
+        with pytest.raises(ValueError, match='overlaps'):
+            call()
+    m, q = _shared(40, 40, kind)
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.mx8_weight_grad(q, D(40, 40), out=m)
+    with pytest.raises(ValueError, match='overlaps'):
+        ops._check_apart('x', [m], [z, q])
+    ops._check_apart('x', [D(40, 40)], [z, q, m])
+
+
+def test_a_weight_gradient_over_its_own_operand_is_refused():
+    for z, q in ((D(8, 8), Q(8, 8)), (Hm(8, 8), Q(8, 8, True))):
+        with pytest.raises(ValueError, match='overlaps'):
+            ops.mx8_weight_grad(q, z, out=z)
+    big = D(20, 8)
+    with pytest.raises(ValueError, match='overlaps'):
+        ops.mx8_weight_grad(Q(8, 8), big.rows(0, 8), out=big.rows(7, 15))
