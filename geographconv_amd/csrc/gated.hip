@@ -65,7 +65,7 @@ struct TileArgs {
     // epilogue
     int mode, out_type, act;
     void* C[2]; int64_t ldc[2];
-    int64_t ncols;                                    // columns to write (N and the pads kept zero)
+    int64_t nc[2], nck[2], ncols;                     // columns to write (N and the pads kept zero): of C, of what is kept in full, the most of all
     const float* bias[2];
     int keep;                                         // EPI_GATED: what is kept of G, U (0, GEOGCN_KEEP_FULL, GEOGCN_KEEP_MX8)
     void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
@@ -403,15 +403,15 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int64_t col = n0 + wn * CW + (jj + h) * 16 + lg * 4;
-                            if (col < a.ncols) {
+                            if (col < a.nc[0]) {
                                 float x[4];
 #pragma unroll
                                 for (int r = 0; r < 4; ++r) x[r] = col + r < a.N ? gate_value(a.act, v[0][h][r]) * v[1][h][r] : 0.f;
                                 store_quad(a.C[0], a.ldc[0], a.out_type, row, col, x);
-                                if (a.keep == GEOGCN_KEEP_FULL) {
-                                    store_quad(a.keepP[0], a.ldk[0], a.out_type, row, col, v[0][h]);
-                                    store_quad(a.keepP[1], a.ldk[1], a.out_type, row, col, v[1][h]);
-                                }
+                            }
+                            if (a.keep == GEOGCN_KEEP_FULL) {
+                                if (col < a.nck[0]) store_quad(a.keepP[0], a.ldk[0], a.out_type, row, col, v[0][h]);
+                                if (col < a.nck[1]) store_quad(a.keepP[1], a.ldk[1], a.out_type, row, col, v[1][h]);
                             }
                         }
                     }
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
             for (int r = 0; r < 4; ++r) x[r] = col + r < a.N ? acc[i][j][r] : 0.f;
             if (a.mode == EPI_SLAB) {
                 if (col < a.segw) *reinterpret_cast<float4*>(a.W + ((int64_t)z * a.M + row) * a.ldw + q * a.segw + col) = make_float4(x[0], x[1], x[2], x[3]);
-            } else if (col < a.ncols) {
+            } else if (col < (q ? a.nc[1] : a.nc[0])) {
                 store_quad(a.C[q], a.ldc[q], a.out_type, row, col, x);
             }
         }
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(const TileArgs a) {
 // 32 columns are one checkpoint block of a row.  Bound by the latency of one round of loads and the reduction: 1 x 1024 -> 4096 in bf16 (16.8 MB)
 // 6.4-7.1 us = 2.4-2.6 TB/s (8.5 + 4.8 us by tiles and a split).
 struct FewArgs {
-    int64_t M, ldx, ldwg, ldwu, ncols;
+    int64_t M, ldx, ldwg, ldwu, ncols, nck[2];        // (columns to write of H and of what is kept in full)
     int K, N, act, out_type, keep;
     const void *X, *Wg, *Wu;
     const float* bias[2];
@@ -590,9 +590,10 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const FewArgs a) {
             else static_cast<uint16_t*>(p)[row * ld + c] = (uint16_t)(pack_bf16(x, 0.f) & 0xffffu);
         };
         const bool in = row < a.M;
-        if (in && c < a.ncols) {
-            put(a.H, a.ldh, h);
-            if (a.keep == GEOGCN_KEEP_FULL) { put(a.keepP[0], a.ldk[0], s[0]); put(a.keepP[1], a.ldk[1], s[1]); }
+        if (in && c < a.ncols) put(a.H, a.ldh, h);
+        if (a.keep == GEOGCN_KEEP_FULL) {
+            if (in && c < a.nck[0]) put(a.keepP[0], a.ldk[0], s[0]);
+            if (in && c < a.nck[1]) put(a.keepP[1], a.ldk[1], s[1]);
         }
         if (a.keep == GEOGCN_KEEP_MX8) {
 #pragma unroll
@@ -612,7 +613,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const FewArgs a) {
 
 // ---- partial products of a split reduction, added in split order, and the epilogue that they were waiting for ---------------------------
 struct FinishArgs {
-    int64_t M, N, segw, ldw, ncols;
+    int64_t M, N, segw, ldw, nc[2], nck[2];           // (TileArgs)
     int nsplit, nseg, mode, out_type, act, keep;
     const float* W;
     void* C[2]; int64_t ldc[2];
@@ -644,21 +645,24 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
             }
         }
         if (a.mode != EPI_GATED) {
-            if (col < a.ncols)
-                for (int q = 0; q < a.nseg; ++q) store_quad(a.C[q], a.ldc[q], a.out_type, row, col, v[q]);
+            for (int q = 0; q < a.nseg; ++q)
+                if (col < a.nc[q]) store_quad(a.C[q], a.ldc[q], a.out_type, row, col, v[q]);
             continue;
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[q][r] = col + r < a.N ? v[q][r] + (a.bias[q] ? a.bias[q][col + r] : 0.f) : 0.f;
-        if (col < a.ncols) {
+        if (col < a.nc[0]) {
             float x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = col + r < a.N ? gate_value(a.act, v[0][r]) * v[1][r] : 0.f;
             store_quad(a.C[0], a.ldc[0], a.out_type, row, col, x);
-            if (a.keep == GEOGCN_KEEP_FULL)
-                for (int q = 0; q < 2; ++q) store_quad(a.keepP[q], a.ldk[q], a.out_type, row, col, v[q]);
+        }
+        if (a.keep == GEOGCN_KEEP_FULL) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                if (col < a.nck[q]) store_quad(a.keepP[q], a.ldk[q], a.out_type, row, col, v[q]);
         }
         if (a.keep == GEOGCN_KEEP_MX8) {
 #pragma unroll
@@ -824,11 +828,11 @@ int64_t out_cols(int type, int64_t N, int64_t ld) { return std::min<int64_t>(ld,
 
 int finish(const TileArgs& t, int nseg, int mode, hipStream_t st) {
     FinishArgs f;
-    f.M = t.M; f.N = t.N; f.segw = t.segw; f.ldw = t.ldw; f.ncols = t.ncols;
+    f.M = t.M; f.N = t.N; f.segw = t.segw; f.ldw = t.ldw;
     f.nsplit = t.nsplit; f.nseg = nseg; f.mode = mode; f.out_type = t.out_type; f.act = t.act; f.keep = t.keep;
     f.W = t.W;
     for (int q = 0; q < 2; ++q) {
-        f.C[q] = t.C[q]; f.ldc[q] = t.ldc[q]; f.bias[q] = t.bias[q];
+        f.C[q] = t.C[q]; f.ldc[q] = t.ldc[q]; f.bias[q] = t.bias[q]; f.nc[q] = t.nc[q]; f.nck[q] = t.nck[q];
         f.keepP[q] = t.keepP[q]; f.ldk[q] = t.ldk[q]; f.keepS[q] = t.keepS[q];
     }
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(t.M * (t.segw / 4), 256), (int64_t)kNumCU * 32);
@@ -994,7 +998,7 @@ template <typename T, int VEC>
 int launch_few(const FewArgs& a, hipStream_t st) {
     const int rm = a.M == 1 ? 1 : a.M == 2 ? 2 : a.M <= 4 ? 4 : 8;
     auto* k = rm == 1 ? &few_rows_kernel<T, VEC, 1> : rm == 2 ? &few_rows_kernel<T, VEC, 2> : rm == 4 ? &few_rows_kernel<T, VEC, 4> : &few_rows_kernel<T, VEC, 8>;
-    const int64_t cols = a.keep == GEOGCN_KEEP_MX8 ? std::max(a.ncols, up(a.N, kMxBlock)) : a.ncols;
+    const int64_t cols = std::max(a.ncols, a.keep == GEOGCN_KEEP_MX8 ? up(a.N, kMxBlock) : std::max(a.nck[0], a.nck[1]));
     hipLaunchKernelGGL(k, dim3((unsigned)cdiv(cols, 32), (unsigned)cdiv(a.M, rm)), dim3(512), 0, st, a);
     GEOGCN_LAUNCH_CHECK("few_rows_kernel");
     return 0;
@@ -1004,23 +1008,34 @@ int forward_few(const FwdArgs& f, hipStream_t st) {
     a.M = f.M; a.K = (int)f.K; a.N = (int)f.N; a.act = f.act; a.out_type = f.type; a.keep = f.keep;
     a.X = f.X.p; a.ldx = f.X.ld; a.Wg = f.Wg.p; a.ldwg = f.Wg.ld; a.Wu = f.Wu.p; a.ldwu = f.Wu.ld;
     a.bias[0] = f.bg; a.bias[1] = f.bu; a.H = f.H; a.ldh = f.ldh; a.ncols = out_cols(f.type, f.N, f.ldh);
-    for (int q = 0; q < 2; ++q) { a.keepP[q] = f.keepP[q]; a.ldk[q] = f.ldk[q]; a.keepS[q] = f.keepS[q]; }
+    for (int q = 0; q < 2; ++q) {
+        a.keepP[q] = f.keepP[q]; a.ldk[q] = f.ldk[q]; a.keepS[q] = f.keepS[q];
+        a.nck[q] = f.keep == GEOGCN_KEEP_FULL ? out_cols(f.type, f.N, f.ldk[q]) : 0;
+    }
     if (f.type == GEOGCN_T_F32) return launch_few<float, 4>(a, st);
     const bool wide = f.Wg.ld % 8 == 0 && f.Wu.ld % 8 == 0 && aligned16(f.Wg.p) && aligned16(f.Wu.p);
     return wide ? launch_few<uint16_t, 8>(a, st) : launch_few<uint16_t, 4>(a, st);
 }
 bool few_rows(const FwdArgs& f) { return f.M <= kFewRows && !(f.type == GEOGCN_T_F32 && f.precision == GEOGCN_GEMM_BF16); }
 
+// what the gated epilogue writes
+void gated_outputs(TileArgs& t, const FwdArgs& f) {
+    t.out_type = f.type; t.act = f.act; t.keep = f.keep;
+    t.bias[0] = f.bg; t.bias[1] = f.bu;
+    t.C[0] = f.H; t.ldc[0] = f.ldh;
+    t.nc[0] = t.ncols = out_cols(f.type, f.N, f.ldh);
+    for (int q = 0; q < 2; ++q) {
+        t.keepP[q] = f.keepP[q]; t.ldk[q] = f.ldk[q]; t.keepS[q] = f.keepS[q];
+        if (f.keep == GEOGCN_KEEP_FULL) t.ncols = std::max(t.ncols, t.nck[q] = out_cols(f.type, f.N, f.ldk[q]));
+    }
+}
 int forward_exact(Arena& ar, const FwdArgs& f, hipStream_t st) {
     // [G | U] by the library's dual product into one slab, the gate by the pass that finishes split reductions
     TileArgs t = tile_args();
     t.M = f.M; t.N = f.N; t.nsplit = 1;
     t.segw = up(f.N, kMxBlock); t.ldw = 2 * t.segw;
     t.W = static_cast<float*>(ar.take(f.M * t.ldw * 4));
-    t.out_type = f.type; t.act = f.act; t.keep = f.keep;
-    t.C[0] = f.H; t.ldc[0] = f.ldh; t.ncols = out_cols(f.type, f.N, f.ldh);
-    t.bias[0] = f.bg; t.bias[1] = f.bu;
-    for (int q = 0; q < 2; ++q) { t.keepP[q] = f.keepP[q]; t.ldk[q] = f.ldk[q]; t.keepS[q] = f.keepS[q]; }
+    gated_outputs(t, f);
     const size_t need = f.K ? geogcn_gemm_dual_workspace_bytes(0, f.M, f.N, f.N, f.K, GEOGCN_GEMM_F32) : 0;
     void* w = ar.take((int64_t)need);
     if (ar.counting) return 0;
@@ -1068,11 +1083,7 @@ int forward(Arena& ar, const FwdArgs& f, hipStream_t st) {
     t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
     t.B[0] = wg.p; t.ldb[0] = wg.ld; t.planeB[0] = wg.plane;
     t.B[1] = wu.p; t.ldb[1] = wu.ld; t.planeB[1] = wu.plane;
-    t.out_type = f.type; t.act = f.act; t.keep = f.keep;
-    t.C[0] = f.H; t.ldc[0] = f.ldh;
-    t.ncols = out_cols(f.type, f.N, f.ldh);
-    t.bias[0] = f.bg; t.bias[1] = f.bu;
-    for (int q = 0; q < 2; ++q) { t.keepP[q] = f.keepP[q]; t.ldk[q] = f.ldk[q]; t.keepS[q] = f.keepS[q]; }
+    gated_outputs(t, f);
     return run_forward(ar, t, P, st);
 }
 
@@ -1130,8 +1141,8 @@ int tn_q8(Arena& ar, const MatIn& X, int64_t M, int64_t K, int64_t N, int nseg, 
     if (ar.counting) return 0;
     TileArgs f = tile_args();
     f.M = K; f.N = N; f.nsplit = t.nsplit; f.W = t.W; f.segw = t.seg_w; f.ldw = t.ldw; f.out_type = GEOGCN_T_F32;
-    f.ncols = up(N, 4);
     for (int q = 0; q < nseg; ++q) {
+        f.nc[q] = up(N, 4);
         t.B[q] = B[q]; t.ldb[q] = ldb; t.N[q] = N;
         f.C[q] = dW[q]; f.ldc[q] = lddw[q];
     }
@@ -1207,7 +1218,7 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
         t.B[0] = wg.p; t.ldb[0] = wg.ld; t.planeB[0] = wg.plane;
         t.B[1] = wu.p; t.ldb[1] = wu.ld; t.planeB[1] = wu.plane;
         for (int q = 0; q < 2; ++q) { t.lda[q] = ldo; t.planeA[q] = plane; }
-        t.out_type = b.type; t.C[0] = b.dX; t.ldc[0] = b.lddx; t.ncols = out_cols(b.type, b.K, b.lddx);
+        t.out_type = b.type; t.C[0] = b.dX; t.ldc[0] = b.lddx; t.nc[0] = t.ncols = out_cols(b.type, b.K, b.lddx);
         if (const int rc = run_input_grad(ar, t, PG, st)) return rc;
     }
     if (b.dW[0]) {
@@ -1217,8 +1228,7 @@ int backward(Arena& ar, const BwdArgs& b, hipStream_t st) {
         t.B[0] = dG; t.B[1] = dU;
         for (int q = 0; q < 2; ++q) { t.ldb[q] = ldo; t.planeB[q] = plane; t.C[q] = b.dW[q]; t.ldc[q] = b.lddw[q]; }
         t.out_type = b.type;
-        t.ncols = std::max(out_cols(b.type, b.N, b.lddw[0]), out_cols(b.type, b.N, b.lddw[1]));
-        if (b.lddw[0] != b.lddw[1]) t.ncols = std::min(out_cols(b.type, b.N, b.lddw[0]), out_cols(b.type, b.N, b.lddw[1]));
+        for (int q = 0; q < 2; ++q) t.ncols = std::max(t.ncols, t.nc[q] = out_cols(b.type, b.N, b.lddw[q]));
         if (const int rc = run_weight_grad(ar, t, PX, PG, 2, st)) return rc;
     }
     return 0;
@@ -1252,7 +1262,7 @@ int weight_grad(Arena& ar, const WgradArgs& w, hipStream_t st) {
     t.M = w.K; t.N = w.N; t.K[0] = w.M;
     t.A[0] = x.p; t.lda[0] = x.ld; t.planeA[0] = x.plane;
     t.B[0] = dz.p; t.ldb[0] = dz.ld; t.planeB[0] = dz.plane;
-    t.C[0] = w.dW; t.ldc[0] = w.lddw; t.out_type = w.type; t.ncols = out_cols(w.type, w.N, w.lddw);
+    t.C[0] = w.dW; t.ldc[0] = w.lddw; t.out_type = w.type; t.nc[0] = t.ncols = out_cols(w.type, w.N, w.lddw);
     return run_weight_grad(ar, t, 1, P, 1, st);
 }
 

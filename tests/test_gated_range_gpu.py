@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from . import gated_reference as R
-from .test_gated_gpu import BF, ENV, EPS, _check, _f64, _mat, _problem, _rand
+from .test_gated_gpu import BF, ENV, EPS, _check, _f64, _forward_bounds, _mat, _problem, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,56 @@ def test_the_largest_pre_activations_stay_finite_in_their_checkpoints(dev, M, K)
     _, kept = ops.gated_dense(*(_mat(a, dev, 'bf16') for a in (X, Wg, Wu)), act=ops.ACT_NONE, keep='mx8')
     got = _f64(ops.mx8_unpack(kept.G))
     assert np.array_equal(got, np.tile(np.clip(R.mx8(Wg[:1].astype(np.float64))[2], -TOP, TOP), (M, 1)))
+
+
+def _poisoned(n, F, ld, dtype, dev):
+    from geographconv_amd import ops
+    t = torch.full((n, ld), float('nan'), dtype=torch.float32 if dtype == 'f32' else torch.bfloat16, device=dev)
+    return (ops.DMat if dtype == 'f32' else ops.HMat)(n, F, t=t)
+
+
+def _check_pads(m, what):
+    """The pad columns of a result: zero up to roundup4 (fp32) / roundup64 or the pitch (bf16), left alone behind."""
+    from geographconv_amd import ops
+    end = ops.pad4(m.F) if isinstance(m, ops.DMat) else min(m.ld, (m.F + 63) // 64 * 64)
+    assert torch.isfinite(m.t[:, :end].float()).all(), what
+    assert (m.t[:, m.F:end] == 0).all() and torch.isnan(m.t[:, end:].float()).all(), what
+
+
+def _forward_into(X, Wg, Wu, act, H, keep, G, U, precision):
+    """The C entry with given matrices for the kept G, U."""
+    from geographconv_amd import _ffi, ops
+    ops._on_device(H.t.get_device(), ops._call_with_ws, _ffi.lib().geogcn_gated_fwd, 'gated_fwd', X.n, X.F, Wg.F, ops._mat_type(X), X.t.data_ptr(), X.ld,
+                   Wg.t.data_ptr(), Wg.ld, Wu.t.data_ptr(), Wu.ld, None, None, act, H.t.data_ptr(), H.ld, ops._KEEP[keep], *ops._mat_args(G),
+                   *ops._mat_args(U), ops.GEMM_PRECISIONS[precision])
+
+
+@pytest.mark.parametrize('M,K', [(5, 70), (300, 70), (40, 4096)])
+def test_kept_matrices_of_other_pitches_have_zero_pads(dev, M, K):
+    """bf16 G and U of wider pitches than H's: their own pads are zero too (a few rows, tiles, a split reduction)."""
+    from geographconv_amd import ops
+    N = 90
+    d, r = _problem(dev, M, K, N, 'bf16', False, M)
+    for lds in ((92, 128, 96), (92, 92, 200), (128, 128, 128)):
+        H, G, U = (_poisoned(M, N, ld, 'bf16', dev) for ld in lds)
+        _forward_into(d['X'], d['Wg'], d['Wu'], ops.ACT_SILU, H, 'full', G, U, 'bf16x3')
+        for m, ref, what in zip((H, G, U), _forward_bounds(r, 'silu', 'bf16'), 'HGU'):
+            _check(_f64(m), ref, what)
+            _check_pads(m, (what, lds))
+
+
+@pytest.mark.parametrize('M', [30, 3000])
+@pytest.mark.parametrize('precision', ['bf16x3', 'bf16'])
+def test_weight_gradients_of_other_pitches_have_zero_pads(dev, M, precision):
+    from geographconv_amd import ops
+    K, N = 70, 90
+    d, r = _problem(dev, M, K, N, 'bf16', False, M)
+    kept = ops.GatedTape(_mat(_rand((M, N), 21), dev, 'bf16'), _mat(_rand((M, N), 22), dev, 'bf16'))
+    dH = _mat(_rand((M, N), 23), dev, 'bf16')
+    want = ops.gated_dense_bwd(dH, d['X'], d['Wg'], d['Wu'], kept, act=ops.ACT_SILU, precision=precision)
+    for lds in ((128, 92), (92, 128), (96, 200)):
+        dX, dWg, dWu = _poisoned(M, K, 72, 'bf16', dev), *(_poisoned(K, N, ld, 'bf16', dev) for ld in lds)
+        ops.gated_dense_bwd(dH, d['X'], d['Wg'], d['Wu'], kept, act=ops.ACT_SILU, dX=dX, dWg=dWg, dWu=dWu, precision=precision)
+        for m, w, what in zip((dX, dWg, dWu), want, ('dX', 'dWg', 'dWu')):
+            assert torch.equal(m.t[:, :m.F], w.t[:, :m.F])
+            _check_pads(m, (what, lds))
