@@ -252,7 +252,8 @@ class DenseLayer(Layer):
     """y = nonlinearity(x . W + b)   (lasagne DenseLayer; the highway gate, gcnmodel.py:285).
 
     ``checkpoint='mx8'`` (dense input, outside the graph product): the tape keeps x in 8 bits (ops.mx8_pack, 1.03 bytes a value) and the
-    weight gradient is taken from the codes; the forward and the input gradient are unchanged."""
+    weight gradient is taken from the codes; the forward and the input gradient are unchanged.  The 4 bytes a value that x took are freed
+    unless another layer's backward reads them too: the layer below, if its activation's gradient is taken from its output."""
 
     early_starts = {'fwd': 0, 'bwd': 0}     # exchanges started ahead of their layer (diagnostics / tests)
 
@@ -379,7 +380,8 @@ class DenseLayer(Layer):
             saved['logits'] = y
             y = K.softmax_rows(y, argmax=amax)
             saved['argmax'] = amax
-        saved['y'] = y
+        if self.nonlinearity.act != 0 or hasattr(self, 'highway_conv') or hasattr(self, 'highway_gate'):
+            saved['y'] = y                # (a linear layer's backward does not read its output: the tape does not hold it)
         if tape is not None:
             tape[self] = saved
         return y
@@ -476,7 +478,7 @@ class DenseLayer(Layer):
         """dS = gradient at the pre-activation, with this layer's bias gradient written on the way (fused into the
         activation-gradient kernel where there is one; skipped when the producer of `grad` already wrote it)."""
         K = backend.active()
-        y = tape[self]['y']
+        y = tape[self].get('y')
         bias_done = isinstance(grad, PreAct) and grad.bias_done
         if isinstance(grad, PreAct):
             dS = grad.m
@@ -607,8 +609,8 @@ class DenseLayer(Layer):
 class GatedDenseLayer(Layer):
     """y = nonlinearity(x . Wg + bg) * (x . Wu + bu): a dense layer whose units each carry a gate of their own (ops.gated_dense; no
     reference counterpart, a sibling of the highway block).  ``nonlinearity``: linear, tanh, sigmoid, rectify, swish or gelu.
-    ``checkpoint='mx8'``: the tape keeps x and the two pre-activations in 8 bits instead of fp32 (3.1 bytes for 12) and the backward runs
-    from the codes."""
+    ``checkpoint='mx8'``: the tape keeps x and the two pre-activations in 8 bits instead of fp32 (1.03 bytes a value instead of 4; x's fp32 values
+    are freed unless another layer's backward reads them, DenseLayer) and the backward runs from the codes."""
 
     def __init__(self, incoming, num_units, Wg=_init.GlorotUniform(), Wu=_init.GlorotUniform(), bg=_init.Constant(0.), bu=_init.Constant(0.),
                  nonlinearity=_nl.sigmoid, name=None, checkpoint=None):
@@ -843,6 +845,7 @@ def get_output(layer_or_layers, inputs=None, tape=None, **kwargs):
         values[ins[0]] = inputs
     started = set()
     kwargs = dict(kwargs, evaluated_layers=frozenset(all_layers))       # (fusions across layers ask whether their partner takes part)
+    lean = any(getattr(l, 'checkpoint', None) is not None for l in all_layers)
     for pos, layer in enumerate(all_layers):
         if layer in values:
             continue
@@ -867,9 +870,8 @@ def get_output(layer_or_layers, inputs=None, tape=None, **kwargs):
                 started.add(nxt)
         values[layer] = layer.forward(x, tape, **kwargs)
     if tape is not None:
-        # (what a checkpointing layer reads is on the tape in 8 bits: the tape does not hold it whole as well)
-        packed = {l.input_layer for l in all_layers if getattr(l, 'checkpoint', None) is not None}
-        tape['__values__'] = {l: v for l, v in values.items() if l not in packed} if packed else values
+        # (the tape of a network that checkpoints layers holds what the backward reads and the values asked for, not every layer's)
+        tape['__values__'] = values if not lean else {l: values[l] for l in (layer_or_layers if hasattr(layer_or_layers, '__iter__') else [layer_or_layers])}
     try:
         return [values[l] for l in layer_or_layers]
     except TypeError:
