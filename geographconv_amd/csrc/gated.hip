@@ -1149,6 +1149,12 @@ int tn_q8(Arena& ar, const MatIn& X, int64_t M, int64_t K, int64_t N, int nseg, 
     if (const int rc = x3_tn_launch(160, bn, t, st)) return rc;
     return finish(f, nseg, EPI_STORE, st);
 }
+// The library's fp32 products leave the pad columns of a result as they are where they add up a split reduction: a result that they form gets its
+// pads (fewer than four columns) from here.
+int zero_pads(void* C, int64_t rows, int64_t cols, int64_t ld, hipStream_t st) {
+    const int64_t pads = up(cols, 4) - cols;
+    return pads ? zero_rows_async(static_cast<float*>(C) + cols, rows, pads, ld, st) : 0;
+}
 // the products by the library's fp32 kernels: dG, dU (and a checkpointed X) as fp32 matrices
 int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
     const int64_t ldo = up(b.N, 4);
@@ -1158,6 +1164,8 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
     if (b.dX) {
         const size_t need = geogcn_gemm_kcat_workspace_bytes(1, b.M, b.K, b.N, b.N, precision);
         void* w = ar.take((int64_t)need);
+        if (!ar.counting)
+            if (const int rc = zero_pads(b.dX, b.M, b.K, b.lddx, st)) return rc;
         if (!ar.counting)
             if (const int rc = geogcn_gemm_kcat_f32(1, b.M, b.K, b.N, b.N, dG, ldo, static_cast<const float*>(b.Wg.p), b.Wg.ld, dU, ldo,
                                                     static_cast<const float*>(b.Wu.p), b.Wu.ld, static_cast<float*>(b.dX), b.lddx, 0, precision,
@@ -1178,6 +1186,8 @@ int backward_exact(Arena& ar, const BwdArgs& b, int precision, hipStream_t st) {
         }
         const size_t need = geogcn_gemm_dual_workspace_bytes(1, b.K, b.N, b.N, b.M, precision);
         void* w = ar.take((int64_t)need);
+        for (int q = 0; q < 2 && !ar.counting; ++q)
+            if (const int rc = zero_pads(b.dW[q], b.K, b.N, b.lddw[q], st)) return rc;
         if (!ar.counting)
             if (const int rc = geogcn_gemm_dual_f32(1, b.K, b.N, b.N, b.M, X, ldx, dG, ldo, dU, ldo, static_cast<float*>(b.dW[0]), b.lddw[0],
                                                     static_cast<float*>(b.dW[1]), b.lddw[1], nullptr, GEOGCN_ACT_NONE, nullptr, GEOGCN_ACT_NONE, precision,
@@ -1242,6 +1252,7 @@ int weight_grad_exact(Arena& ar, const WgradArgs& w, hipStream_t st) {
     void* g = ar.take((int64_t)need);
     if (ar.counting) return 0;
     if (const int rc = geogcn_mx8_unpack(w.M, (int32_t)w.K, GEOGCN_T_F32, static_cast<const uint8_t*>(w.X.p), w.X.ld, w.X.scale, x, ldx, st)) return rc;
+    if (const int rc = zero_pads(w.dW, w.K, w.N, w.lddw, st)) return rc;
     return geogcn_gemm_f32(1, 0, w.K, w.N, w.M, x, ldx, static_cast<const float*>(w.dZ.p), w.dZ.ld, static_cast<float*>(w.dW), w.lddw, nullptr,
                            GEOGCN_ACT_NONE, 0, GEOGCN_GEMM_F32, need ? g : nullptr, need, st);
 }

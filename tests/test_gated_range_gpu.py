@@ -3,7 +3,7 @@ pytest -m gpu).  Bounds: as derived there (ENV * sum|a.b| for a product, half a 
 import numpy as np
 import pytest
 
-from . import gated_reference as R
+from . import gated_reference as R, gated_shapes as S
 from .test_gated_gpu import BF, ENV, EPS, _check, _f64, _forward_bounds, _mat, _problem, _rand
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +129,128 @@ def test_weight_gradients_of_other_pitches_have_zero_pads(dev, M, precision):
         for m, w, what in zip((dX, dWg, dWu), want, ('dX', 'dWg', 'dWu')):
             assert torch.equal(m.t[:, :m.F], w.t[:, :m.F])
             _check_pads(m, (what, lds))
+
+
+# ---- every tile shape, every result ------------------------------------------------------------------------------------------------------------
+# Inputs of the blocks at precision='bf16' are numbers that bf16 holds, so rounding the operands changes nothing and the bounds above stand; dG and
+# dU are not, and are off by half a step (BF).  References: torch's products of 64-bit matrices, on the GPU.
+def _mat_on(gen, n, F, dtype, scale, precision, dev, ld=None):
+    from geographconv_amd import ops
+    v = torch.randn((n, F), generator=gen, device=dev) * scale
+    if precision == 'bf16':
+        v = v.bfloat16().float()
+    ld = ld or (ops.pad4(F) if dtype == 'f32' else ops.bf16_ld(F))
+    t = torch.zeros((n, ld), dtype=torch.float32 if dtype == 'f32' else torch.bfloat16, device=dev)
+    t[:, :F] = v
+    return (ops.DMat if dtype == 'f32' else ops.HMat)(n, F, t=t)
+
+
+def _wide(m):
+    """the values of a matrix or a checkpoint in 64 bits, on the GPU"""
+    from geographconv_amd import ops
+    m = ops.mx8_unpack(m) if isinstance(m, ops.MX8Mat) else m
+    return m.t[:, :m.F].double().contiguous()
+
+
+def _close(got, want, bound, what):
+    got = got.double()
+    assert got.shape == want.shape and torch.isfinite(got).all(), what
+    bad = (got - want).abs() > bound
+    assert not bad.any(), "%s: %d of %d entries out of bounds, worst %.3g x" % (what, bad.sum(), bad.numel(), ((got - want).abs() / bound).max())
+
+
+def _silu(g):
+    s = torch.sigmoid(g)
+    return g * s, s * (1 + g * (1 - s))
+
+
+def _seeded(dev, *sizes):
+    return torch.Generator(device=dev).manual_seed(sum(s * p for s, p in zip(sizes, (1, 3, 7))))
+
+
+@pytest.mark.parametrize('M,K,N,dtype,precision', S.FORWARD)
+def test_forward_on_every_tile_shape(dev, M, K, N, dtype, precision):
+    from geographconv_amd import ops
+    gen = _seeded(dev, M, K, N)
+    X = _mat_on(gen, M, K, dtype, 1.0, precision, dev)
+    Wg, Wu = (_mat_on(gen, K, N, dtype, K ** -0.5, precision, dev) for _ in range(2))
+    b = [torch.randn(N, generator=gen, device=dev) for _ in range(2)]
+    x, wg, wu = _wide(X), _wide(Wg), _wide(Wu)
+    G, U = x @ wg + b[0].double(), x @ wu + b[1].double()
+    eg, eu = (ENV * (x.abs() @ w.abs() + v.double().abs()) for w, v in ((wg, b[0]), (wu, b[1])))
+    v = _silu(G)[0]
+    half = BF if dtype == 'bf16' else 2.0 ** -23
+    h = 1.2 * U.abs() * eg + v.abs() * eu + EPS * v.abs() * U.abs() + EPS * U.abs() + half * (v * U).abs() + 1e-30
+    out = _poisoned(M, N, ops.pad4(N) + 4 if dtype == 'f32' else ops.bf16_ld(N), dtype, dev)
+    H, kept = ops.gated_dense(X, Wg, Wu, *b, act=ops.ACT_SILU, keep='full', precision=precision, out=out)
+    _close(H.t[:, :N], v * U, h, 'H')
+    _check_pads(H, 'H')
+    for m, w, e, what in ((kept.G, G, eg, 'G'), (kept.U, U, eu, 'U')):
+        _close(m.t[:, :N], w, e + half * w.abs() + 1e-30, what)
+        assert (m.t[:, N:ops.pad4(N) if dtype == 'f32' else m.ld] == 0).all(), what
+    H8, k8 = ops.gated_dense(X, Wg, Wu, *b, act=ops.ACT_SILU, keep='mx8', precision=precision)
+    _close(H8.t[:, :N], v * U, h, 'H beside checkpoints')
+    _close(ops.gated_dense(X, Wg, Wu, *b, act=ops.ACT_SILU, precision=precision).t[:, :N], v * U, h, 'H alone')
+    for q, w, e, what in ((k8.G, G, eg, 'G'), (k8.U, U, eu, 'U')):
+        s = torch.exp2(q.scales.double() - 127).repeat_interleave(32, dim=1)[:, :N]
+        got = _wide(q)
+        _close(got, w, torch.maximum(2.0 ** -4 * (w.abs() + e), 2.0 ** -10 * s) * (1 + 1e-6) + e + (BF * w.abs() if dtype == 'bf16' else 0), what + ' in 8 bits')
+        assert (q.codes[:, N:] & 0x7f == 0).all()
+
+
+def _backward_case(dev, M, K, N, dtype, precision, eight):
+    from geographconv_amd import ops
+    gen = _seeded(dev, M, K, N)
+    X = _mat_on(gen, M, K, dtype, 1.0, precision, dev)
+    Wg, Wu = (_mat_on(gen, K, N, dtype, K ** -0.5, precision, dev) for _ in range(2))
+    G, U = (_mat_on(gen, M, N, dtype, 1.0, None, dev) for _ in range(2))
+    dH = _mat_on(gen, M, N, dtype, 1e-3, None, dev)
+    if eight:
+        X, G, U = ops.mx8_pack(X), ops.mx8_pack(G), ops.mx8_pack(U)
+    x, wg, wu, g, u, h = (_wide(m) for m in (X, Wg, Wu, G, U, dH))
+    v, d = _silu(g)
+    dG, dU = h * u * d, h * v
+    eg, eu = EPS * (1 + g.abs()) * (h * u).abs() + 1e-37, EPS * (1 + g.abs()) * h.abs() + 1e-37
+    rnd = ENV + (BF if precision == 'bf16' else 2.0 ** -16 if dtype == 'bf16' else 0)
+    half = BF if dtype == 'bf16' else 2.0 ** -23
+    xt, ax = x.t().contiguous(), x.t().abs().contiguous()
+    want = [(dG @ wg.t().contiguous() + dU @ wu.t().contiguous(),
+             (rnd * dG.abs() + 2 * eg) @ wg.t().abs().contiguous() + (rnd * dU.abs() + 2 * eu) @ wu.t().abs().contiguous()),
+            (xt @ dG, ax @ (rnd * dG.abs() + 2 * eg)), (xt @ dU, ax @ (rnd * dU.abs() + 2 * eu))]
+    want = [(w, (1 + half) * e + half * w.abs() + 1e-30) for w, e in want]
+    want += [(t.sum(0), 128 * 2.0 ** -24 * t.abs().sum(0) + e.sum(0) + 1e-30) for t, e in ((dG, eg), (dU, eu))]
+    ld = lambda F: ops.pad4(F) + 4 if dtype == 'f32' else ops.bf16_ld(F) + 8
+    outs = [_poisoned(n, F, ld(F), dtype, dev) for n, F in ((M, K), (K, N), (K, N))]
+    ops.gated_dense_bwd(dH, X, Wg, Wu, ops.GatedTape(G, U), act=ops.ACT_SILU, dX=outs[0], dWg=outs[1], dWu=outs[2], precision=precision)
+    db = ops.gated_dense_bwd(dH, X, Wg, Wu, ops.GatedTape(G, U), act=ops.ACT_SILU, bias=True, need_input_grad=False, precision=precision)[3:]
+    for m, (w, e), what in zip(outs, want, ('dX', 'dWg', 'dWu')):
+        _close(m.t[:, :m.F], w, e, what)
+        _check_pads(m, what)
+    for t, (w, e), what in zip(db, want[3:], ('dbg', 'dbu')):
+        _close(t[:N], w, e, what)
+
+
+@pytest.mark.parametrize('M,K,N,dtype,precision,eight', S.BACKWARD)
+def test_backward_on_every_tile_shape(dev, M, K, N, dtype, precision, eight):
+    _backward_case(dev, M, K, N, dtype, precision, eight)
+
+
+@pytest.mark.parametrize('eight', [False, True])
+@pytest.mark.parametrize('M,K,N,precision', [(16390, 301, 203, 'bf16x3'), (20000, 193, 65, 'bf16x3'), (70, 45, 33, 'f32'), (16390, 301, 203, 'f32'), (1, 5, 3, 'f32')])
+def test_backward_on_the_librarys_kernels(dev, M, K, N, precision, eight):
+    """... and on the library's whole-rows and A^T.B kernels, and its exact fp32 ones."""
+    _backward_case(dev, M, K, N, 'f32', precision, eight)
+
+
+@pytest.mark.parametrize('M,K,N,dtype,precision', S.WEIGHT + [(16500, 301, 255, 'f32', 'bf16x3'), (100, 901, 637, 'f32', 'bf16x3'), (300, 45, 33, 'f32', 'f32')])
+def test_weight_gradient_on_every_tile_shape(dev, M, K, N, dtype, precision):
+    from geographconv_amd import ops
+    gen = _seeded(dev, M, K, N)
+    X = ops.mx8_pack(_mat_on(gen, M, K, dtype, 1.0, None, dev))
+    dZ = _mat_on(gen, M, N, dtype, 1e-2, precision, dev)
+    x, z = _wide(X).t().contiguous(), _wide(dZ)
+    out = _poisoned(K, N, ops.pad4(N) + 4 if dtype == 'f32' else ops.bf16_ld(N) + 8, dtype, dev)
+    ops.mx8_weight_grad(X, dZ, out=out, precision=precision)
+    want = x @ z
+    _close(out.t[:, :N], want, ENV * (x.abs() @ z.abs()) + (BF if dtype == 'bf16' else 2.0 ** -23) * want.abs() + 1e-30, 'dW')
+    _check_pads(out, 'dW')
