@@ -908,13 +908,12 @@ int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
                                  {64, 128, 32, 2, 2, 0.68, run_tiles<3, 3, false, false, 1, 64, 128, 32, 2, 2, 2, false>}};
     static const Shape bf16[] = {{256, 256, 64, 2, 1, 1.0, run_tiles<1, 1, false, false, 1, 256, 256, 64, 2, 4, 2, false>},
                                  {256, 128, 64, 3, 1, 0.85, run_tiles<1, 1, false, false, 1, 256, 128, 64, 4, 2, 3, false>},
-                                 {128, 128, 64, 2, 2, 0.8, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 2, false>},
                                  {128, 128, 64, 4, 1, 0.75, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 4, false>}};
-    // dG, dU of a bf16 block as two terms (256 x 256 / 256 x 128 / 128 x 128: 8,192 x 1,024 -> 4,096 251 / 277 / 282 us, 60,000 x 600 -> 600
-    // 214 / 250 / 238, 1,000 x 600 -> 600 30 / 23 / 19)
+    // dG, dU of a bf16 block as two terms (256 x 256 / 256 x 128 / 128 x 128: 8,192 x 1,024 -> 4,096 251 / 277 / 289 us, 60,000 x 600 -> 600
+    // 214 / 250 / 233, 9,475 x 300 -> 600 63 / 40 / 25)
     static const Shape two[] = {{256, 256, 32, 3, 1, 1.0, run_tiles<2, 1, false, false, 1, 256, 256, 32, 2, 4, 3, false>},
                                 {256, 128, 32, 3, 1, 0.82, run_tiles<2, 1, false, false, 1, 256, 128, 32, 4, 2, 3, false>},
-                                {128, 128, 32, 2, 2, 0.78, run_tiles<2, 1, false, false, 1, 128, 128, 32, 2, 4, 2, false>}};
+                                {128, 128, 32, 3, 2, 0.78, run_tiles<2, 1, false, false, 1, 128, 128, 32, 2, 4, 3, false>}};
     if (P == 2) return run_best(two, ar, t, t.ncols, 1, 2, st);
     return P == 3 ? run_best(fp32, ar, t, t.ncols, 1, 6, st) : run_best(bf16, ar, t, t.ncols, 1, 1, st);
 }
@@ -925,7 +924,6 @@ int run_weight_grad(Arena& ar, TileArgs& t, int PA, int PB, int nseg, hipStream_
     static const Shape mx8[] = {{160, 160, 32, 2, 1, 1.0, run_tiles<1, 3, true, true, 2, 160, 320, 32, 2, 4, 2, false>},
                                 {128, 128, 32, 2, 1, 0.85, run_tiles<1, 3, true, true, 2, 128, 256, 32, 2, 4, 2, false>}};
     static const Shape bf16[] = {{128, 128, 64, 3, 1, 1.0, run_tiles<1, 1, true, true, 2, 128, 256, 64, 2, 4, 3, false>},
-                                 {128, 64, 64, 2, 2, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 2, 2, false>},
                                  {128, 64, 64, 4, 1, 0.7, run_tiles<1, 1, true, true, 2, 128, 128, 64, 2, 4, 4, false>}};
     // dG, dU of a bf16 block as two terms (128 / 64 columns of each, with the gate pass: 8,192 x 1,024 -> 4,096 330 / 362 us, 4,097 x 1,024 ->
     // 1,536 91 / 88, 440,000 x 300 -> 300 882 / 843)

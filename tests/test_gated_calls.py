@@ -4,6 +4,7 @@ import torch
 
 from geographconv_amd import ops
 
+from . import gated_shapes as S
 from .test_gated import D, Hm, Q
 
 
@@ -45,3 +46,13 @@ def test_a_weight_gradient_over_its_own_operand_is_refused():
     big = D(20, 8)
     with pytest.raises(ValueError, match='overlaps'):
         ops.mx8_weight_grad(Q(8, 8), big.rows(0, 8), out=big.rows(7, 15))
+
+
+def test_the_gpu_tests_run_every_tile_shape():
+    """The sizes that test_gated_range_gpu.py compares reach every entry of csrc/gated.hip's tables, with the reduction whole and split."""
+    t = S.tables()
+    seen = {S.forward(t, *c) for c in S.FORWARD}
+    seen |= {S.input_grad(t, *c[:5]) for c in S.BACKWARD} | {S.weight_grads(t, *c) for c in S.BACKWARD} | {S.weight_grad(t, *c) for c in S.WEIGHT}
+    seen = {(s[0], s[1], s[2] > 1) for s in seen if s}
+    want = {(name, i, split) for name, shapes in t.items() for i in range(len(shapes)) for split in (False, True)}
+    assert seen == want, sorted(want - seen)
