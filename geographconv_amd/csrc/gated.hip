@@ -846,6 +846,9 @@ template <int PA, int PB, bool ASTR, bool BSTR, int NSEG, int BM, int BN, int BK
 int run_tiles(Arena& ar, TileArgs& t, const Cut& c, hipStream_t st) {
     t.n_mt = c.n_mt; t.n_nt = c.n_nt; t.nsplit = c.nsplit; t.steps_per_split = c.steps;
     t.segw = (int64_t)c.n_nt * (BN / NSEG); t.ldw = NSEG * t.segw;
+    // (threads of a launch are counted with 32 bits)
+    GEOGCN_REQUIRE((int64_t)c.n_mt * c.n_nt * c.nsplit < ((int64_t)1 << 32) / (WM * WN * 64), GEOGCN_E_SIZE, "gated: a product of %lld x %lld is too large",
+                   (long long)t.M, (long long)t.N);
     if (c.nsplit > 1) t.W = static_cast<float*>(ar.take((int64_t)c.nsplit * t.M * t.ldw * 4));
     if (ar.counting) return 0;
     t.mode = c.nsplit > 1 ? EPI_SLAB : GATED ? EPI_GATED : EPI_STORE;
@@ -1329,7 +1332,8 @@ extern "C" int geogcn_gated_fwd(int64_t M, int64_t K, int64_t N, int32_t type, c
         }
     }
     Arena count{nullptr};
-    if (!empty) forward(count, f, nullptr);
+    if (!empty)
+        if (const int rc = forward(count, f, nullptr)) return rc;
     if (empty) return 0;
     if (const int rc = check_ws(who, count.used, ws, ws_bytes)) return rc;
     Arena ar{static_cast<unsigned char*>(ws), false};
@@ -1378,7 +1382,8 @@ extern "C" int geogcn_gated_bwd(int64_t M, int64_t K, int64_t N, int32_t type, c
     if (K == 0) { b.dX = nullptr; b.dW[0] = b.dW[1] = nullptr; }
     const bool empty = M == 0 || N == 0;
     Arena count{nullptr};
-    if (!empty) backward(count, b, nullptr);
+    if (!empty)
+        if (const int rc = backward(count, b, nullptr)) return rc;
     if (empty) {                                             // no rows, or no units: sums over nothing
         if (b.dX && M > 0)
             if (const int rc = zero_matrix(dX, type, M, out_cols(type, K, lddx), lddx, st)) return rc;
@@ -1412,7 +1417,8 @@ extern "C" int geogcn_mx8_weight_grad(int64_t M, int64_t K, int64_t N, int32_t t
     }
     WgradArgs w{M, K, N, type, precision, MatIn{GEOGCN_T_MX8, X, ldx, Xs}, MatIn{type, dZ, lddz, nullptr}, dW, lddw};
     Arena count{nullptr};
-    if (!none && M > 0) weight_grad(count, w, nullptr);
+    if (!none && M > 0)
+        if (const int rc = weight_grad(count, w, nullptr)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (none) return 0;
     if (M == 0) return zero_matrix(dW, type, K, out_cols(type, N, lddw), lddw, st);

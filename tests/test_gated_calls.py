@@ -1,8 +1,10 @@
 """Calls of the gated dense block and the 8-bit checkpoints that are turned down on the host, and what their sources state (no GPU)."""
+import ctypes as C
+
 import pytest
 import torch
 
-from geographconv_amd import ops
+from geographconv_amd import _ffi, build, ops
 
 from . import gated_shapes as S
 from .test_gated import D, Hm, Q
@@ -56,3 +58,28 @@ def test_the_gpu_tests_run_every_tile_shape():
     seen = {(s[0], s[1], s[2] > 1) for s in seen if s}
     want = {(name, i, split) for name, shapes in t.items() for i in range(len(shapes)) for split in (False, True)}
     assert seen == want, sorted(want - seen)
+
+
+@pytest.fixture(scope='module')
+def lib():
+    build.build_library()
+    return _ffi.lib()
+
+
+def test_sizes_that_no_launch_holds_are_refused_before_any(lib):
+    """2^31 rows (allowed by the checks of the single sizes) are more blocks of a tile than a launch has: refused when the scratch is asked for, not
+    by the launch itself after others ran."""
+    rows, need = 1 << 31, C.c_size_t(0)
+
+    def fwd(M, type):
+        return lib.geogcn_gated_fwd(M, 4, 4, type, 4096, 4, 4096, 4, 4096, 4, None, None, 5, 4096, 4, 0, None, 0, None, None, 0, None, 1, None, C.byref(need), None)
+
+    def bwd(M, type):
+        return lib.geogcn_gated_bwd(M, 4, 4, type, 4096, 4, type, 4096, 4, None, 4096, 4, 4096, 4, type, 4096, 4, None, 4096, 4, None, 5, 4096, 4, 4096, 4,
+                                    4096, 4, None, None, 1, None, C.byref(need), None)
+    for call in (fwd, bwd):
+        for type in (0, 1):
+            need.value = 0
+            assert call(rows, type) == -2 and b'too large' in lib.geogcn_last_error(), (call, type)
+            assert need.value == 0
+    assert fwd(1 << 24, 0) == _ffi.E_WORKSPACE and bwd(1 << 24, 0) == _ffi.E_WORKSPACE
