@@ -1,8 +1,12 @@
 """Calls of the gated dense block and the 8-bit checkpoints that are turned down on the host, and what their sources state (no GPU)."""
 import ctypes as C
+import os
+import re
 
+import numpy as np
 import pytest
 import torch
+from scipy.special import erfcx
 
 from geographconv_amd import _ffi, build, ops
 
@@ -83,3 +87,13 @@ def test_sizes_that_no_launch_holds_are_refused_before_any(lib):
             assert call(rows, type) == -2 and b'too large' in lib.geogcn_last_error(), (call, type)
             assert need.value == 0
     assert fwd(1 << 24, 0) == _ffi.E_WORKSPACE and bwd(1 << 24, 0) == _ffi.E_WORKSPACE
+
+
+def test_the_normal_distributions_polynomial_has_the_error_it_states():
+    """gate.h, normal_fast: R(t) against exp(z^2) erfc(z), z = |x| / sqrt 2, t = 1 / (1 + 0.3 |x|), with the committed coefficients."""
+    src = open(os.path.join(os.path.dirname(S.SOURCE), 'gate.h')).read()
+    k = [float(v.rstrip('f')) for v in re.search(r'k\[10\] = \{(.*?)\}', src).group(1).split(', ')]
+    stated = float(re.search(r'ten terms t \.\. t\^10, largest error ([0-9.e-]+)', src).group(1))
+    t = np.linspace(1e-6, 1, 1000001)
+    error = np.abs(sum(c * t ** (i + 1) for i, c in enumerate(k)) - erfcx((1 / t - 1) / (0.3 * np.sqrt(2))))
+    assert 0.9 * stated < error.max() <= stated
