@@ -205,9 +205,10 @@ struct HwArgs {
     int* amax = nullptr; // softmax epilogue (HW = 2, geogcn_spmm_csr_softmax_f32): C receives softmax(A.B + bias) row by row, amax
     int softmax = 0;     // (nullable) the first index of each row's maximum
 };
+// (the roundings spelled out: every column has the bits of the separate mixing pass, whatever the compiler would fuse)
 __device__ __forceinline__ float4 highway_mix(const float4 t, const float4 hc, const float4 h) {
-    return make_float4(t.x * hc.x + (1.0f - t.x) * h.x, t.y * hc.y + (1.0f - t.y) * h.y,
-                       t.z * hc.z + (1.0f - t.z) * h.z, t.w * hc.w + (1.0f - t.w) * h.w);
+    return make_float4(fmaf(t.x, hc.x, (1.0f - t.x) * h.x), fmaf(t.y, hc.y, (1.0f - t.y) * h.y),
+                       fmaf(t.z, hc.z, (1.0f - t.z) * h.z), fmaf(t.w, hc.w, (1.0f - t.w) * h.w));
 }
 
 struct XcdRows {
