@@ -8,7 +8,7 @@
 // All three products run on ONE tiled kernel over bf16 TERMS: an fp32 value is the exact sum of three bf16 values, and a product of two
 // fp32 matrices is the sum of its six largest cross products (the dropped ones are O(2^-24)), accumulated in fp32; a bf16 value is one term
 // and so is an 8-bit checkpoint's (4 significant bits), so X^T.dG from a checkpoint costs three cross products instead of six and loses
-// nothing on the way.  fp32 (and 8-bit) operands are written as terms side by side, [row][term][roundup64(cols)], by terms_kernel or by the pass
+// nothing on the way.  dG and dU of a bf16 block, formed in fp32, are two terms.  fp32 (and 8-bit) operands are written as terms side by side, [row][term][roundup64(cols)], by terms_kernel or by the pass
 // that forms them; bf16 matrices whose rows are 16-byte aligned are read in place.
 #include "gate.h"
 #include "gemm_call.h"
@@ -993,7 +993,10 @@ struct FwdArgs {
     void* H; int64_t ldh;
     void* keepP[2]; int64_t ldk[2]; uint8_t* keepS[2];
 };
-// The rows up to which every 8 rows take one more pass over the weights (from L2) instead of term planes and whole tiles.
+// The rows up to which every 8 rows take one more pass over the weights (from L2) instead of term planes and whole tiles.  So / by tiles, us on the
+// GPU, 1, 8, 16, 32, 64 rows: 300 -> 300 fp32 4.6 / 15.4, 7.1 / 15.3, 7.2 / 15.3, 7.3 / 16.8, 7.4 / 17.9; 1,024 -> 4,096 fp32 7.3 / 31.4, 12.7 / 31.8,
+// 12.8 / 31.9, 23.0 / 34.8, 42.9 / 35.6; the same in bf16 6.3 / 14.3, 14.5 / 14.2, 15.0 / 14.0, 27.7 / 15.4, 52.3 / 15.8.  (Few columns under a long
+// reduction fill few CUs: 4,096 -> 1,024 in bf16 is 16.6 / 12.6 at one row and 39.4 / 14.1 at 16.)
 constexpr int64_t kFewRows = 16;
 template <typename T, int VEC>
 int launch_few(const FewArgs& a, hipStream_t st) {
@@ -1017,6 +1020,7 @@ int forward_few(const FwdArgs& f, hipStream_t st) {
     const bool wide = f.Wg.ld % 8 == 0 && f.Wu.ld % 8 == 0 && aligned16(f.Wg.p) && aligned16(f.Wu.p);
     return wide ? launch_few<uint16_t, 8>(a, st) : launch_few<uint16_t, 4>(a, st);
 }
+// (an fp32 block at bf16 products: its operands are to be rounded, and this kernel multiplies the stored values)
 bool few_rows(const FwdArgs& f) { return f.M <= kFewRows && !(f.type == GEOGCN_T_F32 && f.precision == GEOGCN_GEMM_BF16); }
 
 // what the gated epilogue writes

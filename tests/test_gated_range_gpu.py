@@ -254,3 +254,90 @@ def test_weight_gradient_on_every_tile_shape(dev, M, K, N, dtype, precision):
     want = x @ z
     _close(out.t[:, :N], want, ENV * (x.abs() @ z.abs()) + (BF if dtype == 'bf16' else 2.0 ** -23) * want.abs() + 1e-30, 'dW')
     _check_pads(out, 'dW')
+
+
+# ---- calls that the tests of the sizes above do not make -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype,ld', [('f32', 160), ('bf16', 132), ('bf16', 136)])
+@pytest.mark.parametrize('M', [1, 3, 9, 16])
+def test_a_few_rows_with_junk_in_the_pads(dev, M, dtype, ld):
+    """Pitches that allow wide loads and that do not, NaN behind roundup4(F) in every operand, a result among rows that stay as they were."""
+    from geographconv_amd import ops
+    K, N = 70, 90
+    d, r = _problem(dev, M, K, N, dtype, True, 12, ld=ld, junk=True)
+    kind = ops.DMat if dtype == 'f32' else ops.HMat
+    big = torch.full((M + 4, ld), 7.0, dtype=torch.float32 if dtype == 'f32' else torch.bfloat16, device=dev)
+    H, kept = ops.gated_dense(d['X'], d['Wg'], d['Wu'], d['bg'], d['bu'], act=ops.ACT_GELU, keep='full', out=kind(M + 4, N, t=big).rows(2, M + 2))
+    for m, ref in zip((H, kept.G, kept.U), _forward_bounds(r, 'gelu', dtype)):
+        _check(_f64(m), ref, 'H, G, U')
+    assert (big[:2] == 7).all() and (big[M + 2:] == 7).all()
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('M,K,N', [(9, 70, 100), (300, 70, 100), (16400, 200, 100)])
+def test_a_gradient_row_that_is_not_finite_stays_alone(dev, M, K, N, dtype):
+    """An infinity or a NaN in a row of dH reaches that row of dX and no other."""
+    from geographconv_amd import ops
+    d, _ = _problem(dev, M, K, N, dtype, False, 6)
+    kept = ops.GatedTape(_mat(_rand((M, N), 21), dev, dtype), _mat(_rand((M, N), 22), dev, dtype))
+    dH = _mat(_rand((M, N), 23), dev, dtype)
+    want = ops.gated_dense_bwd(dH, d['X'], d['Wg'], d['Wu'], kept)[0]
+    dH.t[3, 5], dH.t[8, 99] = float('inf'), float('nan')
+    got = ops.gated_dense_bwd(dH, d['X'], d['Wg'], d['Wu'], kept)[0]
+    ok = torch.ones(M, dtype=torch.bool, device=dev)
+    ok[[3, 8]] = False
+    assert torch.equal(want.t[ok], got.t[ok])
+    assert not torch.isfinite(got.t[~ok][:, :K].float()).any()
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_matrices_of_more_than_2_31_values(dev, dtype):
+    """8,500,000 x 256 -> 256: every offset passes 32 bits.  The last rows against 64 bits; the weight gradients against 64-bit sums in pieces."""
+    from geographconv_amd import ops
+    M, F = 8_500_000, 256
+    kind, tdt = (ops.DMat, torch.float32) if dtype == 'f32' else (ops.HMat, torch.bfloat16)
+    gen = torch.Generator(device=dev).manual_seed(1)
+
+    def big(scale):
+        t = torch.empty((M, F), dtype=tdt, device=dev)
+        for i in range(0, M, 500_000):
+            t[i:i + 500_000] = torch.randn((min(500_000, M - i), F), generator=gen, device=dev) * scale
+        return kind(M, F, t=t)
+    X, dH = big(1.0), big(1e-3)
+    Wg, Wu = (kind(F, F, t=(torch.randn((F, F), generator=gen, device=dev) / 16).to(tdt)) for _ in range(2))
+    H, kept = ops.gated_dense(X, Wg, Wu, act=ops.ACT_NONE, keep='full')
+    x8 = ops.mx8_pack(X)
+    dX, dWg, dWu, dbg, dbu = ops.gated_dense_bwd(dH, X, Wg, Wu, kept, act=ops.ACT_NONE, bias=True)
+    d8 = ops.mx8_weight_grad(x8, dH)
+    n = 300
+    half = BF if dtype == 'bf16' else 2.0 ** -23
+    rnd = ENV + (2.0 ** -16 if dtype == 'bf16' else 0)
+    wide = lambda m, a, b: m.t[a:b].double()
+    wg, wu = wide(Wg, 0, F), wide(Wu, 0, F)
+    a = M - n
+    x, h, g, u = (wide(m, a, M) for m in (X, dH, kept.G, kept.U))
+    mg, mu = x.abs() @ wg.abs(), x.abs() @ wu.abs()
+    for m, w, mag in ((kept.G, x @ wg, mg), (kept.U, x @ wu, mu)):
+        _close(m.t[a:], w, ENV * mag + half * w.abs() + 1e-30, 'G, U')
+    G, U = x @ wg, x @ wu
+    _close(H.t[a:], G * U, 1.01 * (U.abs() * ENV * mg + G.abs() * ENV * mu) + (half + EPS) * (G * U).abs() + 1e-30, 'H')
+    want = (h * u) @ wg.t().contiguous() + (h * g) @ wu.t().contiguous()
+    mag = (h * u).abs() @ wg.t().abs().contiguous() + (h * g).abs() @ wu.t().abs().contiguous()
+    _close(dX.t[a:], want, (rnd + EPS) * mag + half * want.abs() + 1e-30, 'dX')
+    _close(ops.mx8_unpack(x8).t[a:], x, 2.0 ** -4 * x.abs() + 2.0 ** -10 * 2.0 ** -6, 'checkpoint')
+    sums = [torch.zeros((F, F), dtype=torch.float64, device=dev) for _ in range(6)]
+    cols = [torch.zeros(F, dtype=torch.float64, device=dev) for _ in range(4)]
+    for i in range(0, M, 500_000):
+        j = min(M, i + 500_000)
+        x, h, g, u = (wide(m, i, j) for m in (X, dH, kept.G, kept.U))
+        q = ops.mx8_unpack(ops.MX8Mat(j - i, F, x8.codes[i:j], x8.scales[i:j], dtype == 'bf16')).t.double()
+        for k, (l, r) in enumerate(((x, h * u), (x, h * g), (q, h))):
+            sums[2 * k] += l.t().contiguous() @ r
+            sums[2 * k + 1] += l.t().abs().contiguous() @ r.abs()
+        for k, r in enumerate((h * u, h * g)):
+            cols[2 * k] += r.sum(0)
+            cols[2 * k + 1] += r.abs().sum(0)
+    for k, (m, e) in enumerate(((dWg, rnd), (dWu, rnd), (d8, ENV))):
+        _close(m.t, sums[2 * k], (e + EPS) * sums[2 * k + 1] + half * sums[2 * k].abs(), ('dWg', 'dWu', 'dW from codes')[k])
+    # (partial sums of at most 2,048 rows, then of at most 65,535 / 16 of those: far fewer than 2^12 additions in a row)
+    for k, t in enumerate((dbg, dbu)):
+        _close(t[:F], cols[2 * k], 2.0 ** 12 * 2.0 ** -24 * cols[2 * k + 1], 'bias')
