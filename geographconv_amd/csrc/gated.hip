@@ -912,10 +912,9 @@ int run_input_grad(Arena& ar, TileArgs& t, int P, hipStream_t st) {
     static const Shape bf16[] = {{256, 256, 64, 2, 1, 1.0, run_tiles<1, 1, false, false, 1, 256, 256, 64, 2, 4, 2, false>},
                                  {256, 128, 64, 3, 1, 0.85, run_tiles<1, 1, false, false, 1, 256, 128, 64, 4, 2, 3, false>},
                                  {128, 128, 64, 4, 1, 0.75, run_tiles<1, 1, false, false, 1, 128, 128, 64, 2, 4, 4, false>}};
-    // dG, dU of a bf16 block as two terms (256 x 256 / 256 x 128 / 128 x 128: 8,192 x 1,024 -> 4,096 251 / 277 / 289 us, 60,000 x 600 -> 600
-    // 214 / 250 / 233, 9,475 x 300 -> 600 63 / 40 / 25)
+    // dG, dU of a bf16 block as two terms (256 x 256 / 128 x 128: 8,192 x 1,024 -> 4,096 250 / 288 us, 60,000 x 600 -> 600 214 / 230, 9,475 x 300 ->
+    // 600 63 / 25; 256 x 128 lies between them: 275, 251, 40)
     static const Shape two[] = {{256, 256, 32, 3, 1, 1.0, run_tiles<2, 1, false, false, 1, 256, 256, 32, 2, 4, 3, false>},
-                                {256, 128, 32, 3, 1, 0.82, run_tiles<2, 1, false, false, 1, 256, 128, 32, 4, 2, 3, false>},
                                 {128, 128, 32, 3, 2, 0.78, run_tiles<2, 1, false, false, 1, 128, 128, 32, 2, 4, 3, false>}};
     if (P == 2) return run_best(two, ar, t, t.ncols, 1, 2, st);
     return P == 3 ? run_best(fp32, ar, t, t.ncols, 1, 6, st) : run_best(bf16, ar, t, t.ncols, 1, 1, st);
