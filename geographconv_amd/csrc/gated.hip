@@ -52,9 +52,9 @@ __global__ __launch_bounds__(256) void terms_kernel(const TermsJobs jobs) {
 // read as 16-byte fragments, a k-strided one through the transposing LDS read (4 k-values of a lane's own column).  Both images are
 // permuted in 16-byte pieces so that the lanes of a read phase meet different banks.
 // NSEG = 2: the block's columns are BN / 2 of B[0] and the same BN / 2 of B[1] -- a lane then owns g and u of one element.
-// What bounds it: in bf16 the LDS (a wave's 64 x 64 products of a k-step take 256 clocks of its SIMD and 8 KB of reads; two blocks a CU cover each
-// other's barriers) -- 1.17 PFLOP/s at 16,384 x 4,096 -> 4,096, 1.05 at 8,192 x 2,048 -> 8,192, matrix pipe busy 38-56 %, no bank conflicts; at three
-// terms the clock under power (the products of 60,000 x 600 -> 600: 1.0 PFLOP/s) or, with few tiles, a load's latency per stage.
+// What bounds it: large products power and the barriers of the stages (8,192 x 2,048 -> 8,192 in bf16, 1.05 PFLOP/s: 1.8-2.1 GHz, the matrix pipe
+// busy 52 % of the clocks, LDS 26 % and without conflicts, waves waiting 36 %), products of few tiles a load's latency per stage (9,475 x 300 ->
+// 600 in fp32: matrix pipe 31 %, LDS 12 %).  Counters: profiles/gated_block_kernels.md.
 struct TileArgs {
     int64_t M, N;                                     // rows of C, columns of each segment of C
     int n_mt, n_nt, nsplit, steps_per_split;
@@ -861,7 +861,8 @@ int run_tiles(Arena& ar, TileArgs& t, const Cut& c, hipStream_t st) {
 // of them at a time: it takes the products of R tiles at 0.7 of the matrix pipe's rate times the shape's measured standing (`eff`: 1 for the
 // fastest of its list on a large product), or, where few blocks are there to cover for each other, a load's latency (1,900) for every
 // stage that is not asked for ahead; a tile begins and ends in 6,000.  A split writes and reads its slabs (1,500 bytes a clock) and
-// takes one more launch.
+// takes one more launch.  (The constants are fitted to sweeps of the shapes over 100 to 440,000 rows and widths of 256 to 4,096; the estimate errs by
+// up to 15 % where it takes a shape that is not the fastest: the input gradient of 512 x 4,096 -> 4,096 in two terms 82 us, 73 on 256 x 256.)
 struct Shape {
     int bm, bns, bk, stages, per_cu;
     double eff;

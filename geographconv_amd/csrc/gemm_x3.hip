@@ -340,7 +340,7 @@ __global__ __launch_bounds__(TPB, 2) void x3_rows_kernel(const X3RowsArgs a) {
 constexpr int BKH = 32, ROWB = 80;      // k per stage = one MFMA depth; bytes per LDS row: 32 bf16 + 16 B pad (an odd multiple of 16)
 
 // Q8: A is an 8-bit checkpoint (mx8.h).  Its values are one bf16 term each, read as codes (a dword a row of the patch) and scale bytes: three
-// products instead of six, one image of A instead of three (440,000 x 300, 2 x 300 columns: 0.65 ms against 0.97-1.01).
+// products instead of six, one image of A instead of three (440,000 x 300, 2 x 300 columns: 0.60-0.65 ms against 0.97-1.01).
 template <int BM, int BN, bool Q8 = false>
 __global__ __launch_bounds__(512, 1) void x3_tn_kernel(const X3TnCall a) {
     constexpr int NTH = 512, kASplit = 192;                  // threads [0,192): A patches, [192,512): B patches
