@@ -8,8 +8,8 @@
 // All three products run on ONE tiled kernel over bf16 TERMS: an fp32 value is the exact sum of three bf16 values, and a product of two
 // fp32 matrices is the sum of its six largest cross products (the dropped ones are O(2^-24)), accumulated in fp32; a bf16 value is one term
 // and so is an 8-bit checkpoint's (4 significant bits), so X^T.dG from a checkpoint costs three cross products instead of six and loses
-// nothing on the way.  dG and dU of a bf16 block, formed in fp32, are two terms.  fp32 (and 8-bit) operands are written as terms side by side, [row][term][roundup64(cols)], by terms_kernel or by the pass
-// that forms them; bf16 matrices whose rows are 16-byte aligned are read in place.
+// nothing on the way.  dG and dU of a bf16 block, formed in fp32, are two terms.  fp32 (and 8-bit) operands are written as terms side by side,
+// [row][term][roundup64(cols)], by terms_kernel or by the pass that forms them; bf16 matrices whose rows are 16-byte aligned are read in place.
 #include "gate.h"
 #include "gemm_call.h"
 #include "mx8.h"
@@ -892,7 +892,7 @@ int run_best(const Shape (&shapes)[N], Arena& ar, TileArgs& t, int64_t cols, int
 }
 
 // X.[Wg | Wu] and the gate.  (Shapes of two blocks a CU where LDS and registers allow: one block's epilogue and barriers run under the other's
-// products.  8192 x 2048 -> 8192 in bf16: 128 x 256 531-660 us by box, the same with 64 k-values a stage and one block a CU 650-790.)
+// products.  8192 x 2048 -> 8192 in bf16: 128 x 256 524-660 us from machine to machine, the same with 64 k-values a stage and one block a CU 650-790.)
 int run_forward(Arena& ar, TileArgs& t, int P, hipStream_t st) {
     static const Shape fp32[] = {{128, 128, 32, 2, 1, 1.0, run_tiles<3, 3, false, true, 2, 128, 256, 32, 2, 4, 2, true>},
                                  {256, 64, 32, 2, 1, 0.95, run_tiles<3, 3, false, true, 2, 256, 128, 32, 4, 2, 2, true>},

@@ -511,8 +511,8 @@ int geogcn_mx8_unpack(int64_t n, int32_t F, int32_t type, const uint8_t* codes, 
  * type: GEOGCN_T_F32 or GEOGCN_T_BF16, that of every matrix; bg, bu: fp32, may be NULL (each on its own).  Products of fp32 matrices:
  * GEOGCN_GEMM_F32 (the exact fp32 kernels, in launches of their own), GEOGCN_GEMM_BF16X3 (three bf16 terms a value, fp32-class) or
  * GEOGCN_GEMM_BF16 (operands rounded to bf16); accumulation fp32.  (An infinity, or a value from 3.39e38 on, is not the sum of three bf16
- * terms: under BF16X3 its row gives NaN.)  Calls of up to 16 rows multiply in plain fp32 under either of the first two.  The forward products of bf16 matrices are exact
- * products accumulated in fp32, whatever `precision` says.
+ * terms: under BF16X3 its row gives NaN.)  Calls of up to 16 rows multiply in plain fp32 under either of the first two.  The forward products
+ * of bf16 matrices are exact products accumulated in fp32, whatever `precision` says.
  * keep: what of G = X.Wg + bg and U = X.Wu + bu is stored for the backward -- nothing, in the block's type (pitch >= H's), or as 8-bit
  * checkpoints (codes G / U with pitch ldg / ldu and scales Gs / Us as geogcn_mx8_pack writes them).
  * K, N <= 2^20, pitches <= 2^21.  H, G, U, dX, dWg, dWu overlap none of the other matrices.

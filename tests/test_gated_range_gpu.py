@@ -341,3 +341,27 @@ def test_matrices_of_more_than_2_31_values(dev, dtype):
     # (partial sums of at most 2,048 rows, then of at most 65,535 / 16 of those: far fewer than 2^12 additions in a row)
     for k, t in enumerate((dbg, dbu)):
         _close(t[:F], cols[2 * k], 2.0 ** 12 * 2.0 ** -24 * cols[2 * k + 1], 'bias')
+
+
+@pytest.mark.parametrize('M,K,N,precision', [(5, 70, 91, 'bf16x3'), (300, 70, 91, 'bf16x3'), (16385, 301, 257, 'bf16x3'), (33000, 70, 645, 'bf16x3'), (300, 70, 91, 'f32'),
+                                             (17000, 45, 33, 'f32'), (300, 70, 91, 'bf16'), (40, 2500, 91, 'bf16x3')])
+def test_fp32_results_of_every_forward_route_have_zero_pads(dev, M, K, N, precision):
+    """A few rows, tiles, split reductions, the library's whole-rows and exact kernels: H, G and U into matrices full of NaN."""
+    from geographconv_amd import ops
+    gen = _seeded(dev, M, K, N)
+    X = _mat_on(gen, M, K, 'f32', 1.0, precision, dev)
+    Wg, Wu = (_mat_on(gen, K, N, 'f32', K ** -0.5, precision, dev) for _ in range(2))
+    x, wg, wu = _wide(X), _wide(Wg), _wide(Wu)
+    G, U = x @ wg, x @ wu
+    eg, eu = ENV * (x.abs() @ wg.abs()), ENV * (x.abs() @ wu.abs())
+    v = _silu(G)[0]
+    out = [_poisoned(M, N, ops.pad4(N) + e, 'f32', dev) for e in (4, 8, 4)]
+    _forward_into(X, Wg, Wu, ops.ACT_SILU, out[0], 'full', out[1], out[2], precision)
+    h = 1.2 * U.abs() * eg + v.abs() * eu + EPS * v.abs() * U.abs() + EPS * U.abs() + 1e-30
+    for m, w, e, what in zip(out, (v * U, G, U), (h, eg, eu), 'HGU'):
+        _close(m.t[:, :N], w, e + 2.0 ** -23 * w.abs() + 1e-30, what)
+        _check_pads(m, what)
+    H = _poisoned(M, N, ops.pad4(N), 'f32', dev)
+    ops.gated_dense(X, Wg, Wu, act=ops.ACT_SILU, out=H, precision=precision)
+    _close(H.t[:, :N], v * U, h + 2.0 ** -23 * (v * U).abs(), 'H alone')
+    assert (H.t[:, N:] == 0).all()
